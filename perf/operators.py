@@ -47,7 +47,7 @@ def listed():
         _attn("attend", "attend-prompt-8bit", 2, 509, 16, 2, 128, 8, 32, 7000),
         _attn("attend", "attend-long-8bit", 1, 8, 24, 4, 256, 8, 64, 131071),
         _attn("shared", "shared-few-bf16", 4, 1, 8, 2, 64, 16, 0, 61, prefix=515),
-        _attn("shared", "shared-batch-8bit", 32, 1, 24, 4, 128, 8, 64, 250, prefix=8190),
+        _attn("shared", "shared-batch-8bit", 32, 1, 20, 4, 128, 8, 64, 250, prefix=8190),
         _attn("shared", "shared-large-bf16", 64, 4, 24, 4, 256, 16, 0, 200, prefix=32768),
         _lp("logprobs-block-bf16", 8, 248320, 0, "bfloat16", 1, 20),
         _lp("logprobs-batch-fp32", 61, 50021, 3, "float32", 2, 5),
