@@ -6,3 +6,6 @@
 #include "tp.cu"
 #include "stack.cu"
 #include "stack_driver.cu"
+#include "kv_cache.cu"
+#include "attn_batch.cu"
+#include "logprobs.cu"

@@ -65,6 +65,9 @@ EXPORTED = (
     # the verify stack as one object
     "dflash_stack_create", "dflash_stack_forward", "dflash_stack_verify", "dflash_stack_commit",
     "dflash_stack_advance", "dflash_stack_context", "dflash_stack_output", "dflash_stack_destroy",
+    # include/dflash_batch.h: batches of sequences, quantised caches, a shared prefix, log probabilities
+    "dflash_stack_attn_prep_batch", "dflash_stack_kv_read", "dflash_stack_kv_write", "dflash_stack_kv_compact_batch",
+    "dflash_stack_attn_decode_batch", "dflash_stack_attn_decode_batch_workspace_bytes", "dflash_logprobs",
 )
 
 
@@ -78,6 +81,7 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _sz = ctypes.c_size_t
 _f = ctypes.c_float
+_ll = ctypes.c_longlong
 
 
 def _load() -> ctypes.CDLL:
@@ -150,6 +154,14 @@ def _load() -> ctypes.CDLL:
         "dflash_stack_context": ([_vp], _i),
         "dflash_stack_output": ([_vp], _vp),
         "dflash_stack_destroy": ([_vp], None),
+        "dflash_stack_attn_prep_batch": ([_vp, _ll, _vp, _vp, _vp, _ll, _vp, _vp, _i, _i, _i, _i, _f, _f, _vp, _vp], _i),
+        "dflash_stack_kv_read": ([_vp, _vp, _i, _vp, _vp, _vp], _i),
+        "dflash_stack_kv_write": ([_vp, _vp, _i, _vp, _vp, _vp], _i),
+        "dflash_stack_kv_compact_batch": ([_vp, _vp, _vp, _vp, _i, _vp], _i),
+        "dflash_stack_attn_decode_batch_workspace_bytes": ([_vp, _i, _i, _i], _sz),
+        "dflash_stack_attn_decode_batch": ([_vp, _ll, _vp, _ll, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _vp, _vp, _sz, _vp],
+                                           _i),
+        "dflash_logprobs": ([_vp, _i, _ll, _i, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp], _i),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -732,6 +744,275 @@ def accept_reduce(exchange: PeerExchange, set_: int, proposals, tokens=None, acc
     check(lib.dflash_accept_reduce(exchange.ptr, exchange.world, int(set_), _ptr(proposals), drafts, _ptr(tokens),
                                    _ptr(accepted), _stream(stream)))
     return tokens, accepted
+
+
+# ----------------------------------------------------------------------------- batches of sequences
+# (include/dflash_batch.h).  A call on tensors of a device that is not the current one, or with
+# `stream`, is made with that device and stream current: its outputs and workspace then come
+# from that stream's memory.
+
+class KVCacheDesc(ctypes.Structure):
+    """dflash_kv_cache."""
+    _fields_ = [("k", _vp), ("k_scales", _vp), ("k_biases", _vp), ("v", _vp), ("v_scales", _vp), ("v_biases", _vp),
+                ("sequences", _i), ("kv_heads", _i), ("max_len", _i), ("head_dim", _i), ("bits", _i), ("group", _i)]
+
+
+class KVCache:
+    """The attention caches of `sequences` sequences: bits 16 (bf16 rows), or 8 / 4 (affine
+    codes with a bf16 scale and bias per `group` elements, the packed layout of the weights).
+    k and v are (data, scales, biases), data bf16 [sequences, kv_heads, max_len, head_dim] or
+    int32 [sequences, kv_heads, max_len, head_dim * bits / 32]."""
+
+    def __init__(self, sequences: int, kv_heads: int, max_len: int, head_dim: int, bits: int = 16, group: int = 64,
+                 device=None):
+        import torch
+        dev = device or "cuda"
+
+        def one():
+            lead = (sequences, kv_heads, max_len)
+            if bits == 16:
+                return torch.zeros(*lead, head_dim, dtype=torch.bfloat16, device=dev), None, None
+            if bits not in (4, 8) or group not in (32, 64, 128) or head_dim % group:
+                raise DFlashError(DFLASH_ERR_UNSUPPORTED, f"a {bits}-bit cache in groups of {group} of {head_dim}")
+            return (torch.zeros(*lead, head_dim * bits // 32, dtype=torch.int32, device=dev),
+                    torch.zeros(*lead, head_dim // group, dtype=torch.bfloat16, device=dev),
+                    torch.zeros(*lead, head_dim // group, dtype=torch.bfloat16, device=dev))
+
+        self._bind(one(), one(), bits, group)
+
+    @classmethod
+    def of(cls, k, v, bits: int, group: int = 64) -> "KVCache":
+        """A cache over tensors that exist: k and v (data, scales, biases), referenced."""
+        self = cls.__new__(cls)
+        self._bind(k, v, bits, group)
+        return self
+
+    def _bind(self, k, v, bits, group):
+        import torch
+        data = k[0]
+        if data.dim() != 4:
+            raise ValueError(f"cache data of shape {tuple(data.shape)}: [sequences, kv_heads, max_len, ...] is expected")
+        lead = tuple(data.shape[:3])
+        head_dim = data.shape[3] if bits == 16 else data.shape[3] * 32 // bits
+        for d, s, b in (k, v):
+            if d.dtype != (torch.bfloat16 if bits == 16 else torch.int32) or tuple(d.shape) != tuple(data.shape):
+                raise ValueError(f"cache data {d.dtype} {tuple(d.shape)} does not fit a {bits}-bit cache like {tuple(data.shape)}")
+            parts = (d,) if bits == 16 else (d, s, b)
+            for t in parts[1:]:
+                if t is None or t.dtype != torch.bfloat16 or tuple(t.shape) != lead + (head_dim // group,):
+                    raise ValueError(f"a {bits}-bit cache needs bf16 scales and biases {lead + (head_dim // group,)}")
+            if any(not t.is_contiguous() or t.device != data.device for t in parts):
+                raise ValueError("the tensors of a cache must be contiguous and on one device")
+        self.k, self.v, self.bits, self.group = tuple(k), tuple(v), int(bits), int(group) if bits != 16 else 0
+        (self.sequences, self.kv_heads, self.max_len), self.head_dim = lead, int(head_dim)
+        self.device = data.device
+        p = [_ptr(t) for t in (self.k if bits != 16 else (k[0], None, None)) + (self.v if bits != 16 else (v[0], None, None))]
+        self.desc = KVCacheDesc(*p, *lead, self.head_dim, self.bits, self.group)
+        self.ref = ctypes.addressof(self.desc)
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in self.k + self.v if t is not None)
+
+
+def _elsewhere(device, stream):
+    """The context in which a call on tensors of `device` has to run, or None for the current one."""
+    import torch
+    if device.type != "cuda":
+        raise ValueError(f"tensors on {device}: the library runs on CUDA devices only")
+    if stream is not None:
+        return torch.cuda.stream(stream)
+    if device.index != torch.cuda.current_device():
+        return torch.cuda.device(device)
+    return None
+
+
+def _rows_bf16(name, t, device, cols=None):
+    """Checks rows of bf16 whose elements are adjacent."""
+    import torch
+    if t.dtype != torch.bfloat16 or t.dim() != 2 or t.stride(1) != 1 or t.device != device or (
+            cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{name}: bf16 rows on {device} with adjacent elements are expected, got {t.dtype} "
+                         f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
+
+
+def _ints(name, t, device, shape):
+    import torch
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name}: contiguous int32 {shape} on {device} is expected, got {t.dtype} {tuple(t.shape)} on "
+                         f"{t.device}")
+
+
+def _block_tokens(name, rows: int, cache: KVCache) -> int:
+    if rows == 0 or rows % cache.sequences:
+        raise ValueError(f"{name}: {rows} rows for {cache.sequences} sequences")
+    return rows // cache.sequences
+
+
+def stack_attn_prep_batch(qkv, q_norm, k_norm, cache: KVCache, lengths, hq: int, rot: int, eps: float, theta: float,
+                          q_out=None, position0: int = 0, parents=None, stream=None):
+    """Norm and rotary embedding of every sequence's block rows; k and v go to the cache in its
+    format at rows lengths[b] + t, the q heads to q_out bf16 [rows, hq * d] (returned).  qkv
+    rows [q | gate | k | v], row b * T + t being token t of sequence b; lengths int32
+    [sequences] on the device (negative: the sequence takes no part); parents int32
+    [sequences, T]: each block is a tree."""
+    import torch
+    ctx = _elsewhere(cache.device, stream)
+    if ctx is not None:
+        with ctx:
+            return stack_attn_prep_batch(qkv, q_norm, k_norm, cache, lengths, hq, rot, eps, theta, q_out, position0,
+                                         parents)
+    dev, d = cache.device, cache.head_dim
+    T = _block_tokens("qkv", qkv.shape[0], cache)
+    _rows_bf16("qkv", qkv, dev)
+    if qkv.shape[1] < (2 * hq + 2 * cache.kv_heads) * d:
+        raise ValueError(f"qkv rows of {qkv.shape[1]} elements for {hq} q heads and {cache.kv_heads} kv heads of {d}")
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w.dtype != torch.bfloat16 or tuple(w.shape) != (d,) or w.stride(0) != 1 or w.device != dev:
+            raise ValueError(f"{name}: bf16 [{d}] on {dev} is expected")
+    _ints("lengths", lengths, dev, (cache.sequences,))
+    if parents is not None:
+        _ints("parents", parents, dev, (cache.sequences, T))
+    if q_out is None:
+        q_out = torch.empty((qkv.shape[0], hq * d), dtype=torch.bfloat16, device=dev)
+    else:
+        _rows_bf16("q_out", q_out, dev)
+        if q_out.shape[0] != qkv.shape[0] or q_out.shape[1] < hq * d:
+            raise ValueError(f"q_out {tuple(q_out.shape)} for {qkv.shape[0]} rows of {hq * d}")
+    check(lib.dflash_stack_attn_prep_batch(_ptr(qkv), qkv.stride(0), _ptr(q_norm), _ptr(k_norm), _ptr(q_out),
+                                           q_out.stride(0), cache.ref, _ptr(lengths), T, hq, rot, position0, eps, theta,
+                                           _ptr(parents), _stream()))
+    return q_out
+
+
+def stack_attn_decode_batch(q, cache: KVCache, lengths, scale: float, out=None, gate=None,
+                            prefix: Optional[KVCache] = None, prefix_len: Optional[int] = None, parents=None,
+                            workspace=None, stream=None):
+    """out bf16 [rows, hq * d] = softmax(scale q K^T) V (times sigmoid(gate)), token t of
+    sequence b attending to the first prefix_len rows of `prefix` (a cache of one sequence that
+    all share; default: all of it) and to rows 0 .. lengths[b] + t of its own cache, or its
+    path with parents.  workspace: a uint8 tensor of stack_attn_decode_batch_workspace_bytes(),
+    allocated for the call when not given; calls that may overlap, captured graphs included,
+    need one each."""
+    import torch
+    ctx = _elsewhere(cache.device, stream)
+    if ctx is not None:
+        with ctx:
+            return stack_attn_decode_batch(q, cache, lengths, scale, out, gate, prefix, prefix_len, parents, workspace)
+    dev, d = cache.device, cache.head_dim
+    rows, width = q.shape
+    T = _block_tokens("q", rows, cache)
+    _rows_bf16("q", q, dev)
+    hq = width // d
+    if hq * d != width:
+        raise ValueError(f"q rows of {width} elements are no whole number of heads of {d}")
+    if gate is not None:
+        _rows_bf16("gate", gate, dev, width)
+        if gate.shape[0] != rows:
+            raise ValueError(f"gate of {gate.shape[0]} rows for {rows}")
+    _ints("lengths", lengths, dev, (cache.sequences,))
+    if parents is not None:
+        _ints("parents", parents, dev, (cache.sequences, T))
+    if out is None:
+        out = torch.empty((rows, width), dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (rows, width) or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out: contiguous bf16 {(rows, width)} on {dev} is expected")
+    if prefix is not None and prefix.device != dev:
+        raise ValueError(f"the prefix is on {prefix.device}, the cache on {dev}")
+    if prefix_len is None:
+        prefix_len = prefix.max_len if prefix is not None else 0
+    if workspace is None:
+        workspace = torch.empty(stack_attn_decode_batch_workspace_bytes(cache, prefix_len, T, hq), dtype=torch.uint8,
+                                device=dev)
+    check(lib.dflash_stack_attn_decode_batch(
+        _ptr(q), q.stride(0), _ptr(gate), 0 if gate is None else gate.stride(0), cache.ref, _ptr(lengths),
+        None if prefix is None else prefix.ref, prefix_len, _ptr(out), T, hq, scale, _ptr(parents),
+        _ptr(workspace), workspace.numel() * workspace.element_size(), _stream()))
+    return out
+
+
+def stack_attn_decode_batch_workspace_bytes(cache: KVCache, prefix_len: int, tokens: int, hq: int) -> int:
+    return int(lib.dflash_stack_attn_decode_batch_workspace_bytes(cache.ref, prefix_len, tokens, hq))
+
+
+def stack_kv_read(cache: KVCache, rows: int, starts=None, k=None, v=None, stream=None):
+    """Cache rows starts[b] .. starts[b] + rows - 1 of every sequence (starts int32 [sequences]
+    on the device; None: from row 0) as bf16 k, v [sequences, kv_heads, rows, head_dim]."""
+    import torch
+    ctx = _elsewhere(cache.device, stream)
+    if ctx is not None:
+        with ctx:
+            return stack_kv_read(cache, rows, starts, k, v)
+    shape = (cache.sequences, cache.kv_heads, rows, cache.head_dim)
+    if starts is not None:
+        _ints("starts", starts, cache.device, (cache.sequences,))
+    k, v = (torch.empty(shape, dtype=torch.bfloat16, device=cache.device) if t is None else t for t in (k, v))
+    _cache_rows(k, v, shape, cache.device)
+    check(lib.dflash_stack_kv_read(cache.ref, _ptr(starts), rows, _ptr(k), _ptr(v), _stream()))
+    return k, v
+
+
+def _cache_rows(k, v, shape, device):
+    import torch
+    for t in (k, v):
+        if t.dtype != torch.bfloat16 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"cache rows: contiguous bf16 {shape} on {device} are expected, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+
+
+def stack_kv_write(cache: KVCache, k, v, starts=None, stream=None):
+    """Rows k, v (bf16 [sequences, kv_heads, rows, head_dim], already normalised and rotated)
+    into the cache in its format, from row starts[b] (None: 0) on."""
+    ctx = _elsewhere(cache.device, stream)
+    if ctx is not None:
+        with ctx:
+            return stack_kv_write(cache, k, v, starts)
+    _cache_rows(k, v, (cache.sequences, cache.kv_heads, k.shape[2], cache.head_dim), cache.device)
+    if starts is not None:
+        _ints("starts", starts, cache.device, (cache.sequences,))
+    check(lib.dflash_stack_kv_write(cache.ref, _ptr(starts), k.shape[2], _ptr(k), _ptr(v), _stream()))
+
+
+def stack_kv_compact_batch(cache: KVCache, lengths, rows, counts, stream=None):
+    """After a tree round: cache rows lengths[b] + rows[b, i] -> lengths[b] + i for i < counts[b]
+    (int32 on the device: rows [sequences, <= 32], lengths and counts [sequences])."""
+    ctx = _elsewhere(cache.device, stream)
+    if ctx is not None:
+        with ctx:
+            return stack_kv_compact_batch(cache, lengths, rows, counts)
+    _ints("lengths", lengths, cache.device, (cache.sequences,))
+    _ints("counts", counts, cache.device, (cache.sequences,))
+    _ints("rows", rows, cache.device, (cache.sequences, rows.shape[-1]))
+    check(lib.dflash_stack_kv_compact_batch(cache.ref, _ptr(lengths), _ptr(rows), _ptr(counts), rows.shape[1], _stream()))
+
+
+LOGITS_BF16, LOGITS_FP32 = 0, 1
+
+
+def logprobs(logits, tokens=None, top: int = 0, stream=None) -> dict:
+    """Log probabilities of rows of logits (bf16 or fp32 [rows, vocab], adjacent elements):
+    {"logprobs": fp32 [rows, n] at tokens (int32 [rows, n]; 0 for a negative token, NaN for one
+    past the vocabulary), "entropy": fp32 [rows], "top_ids": int32 [rows, top], "top_logprobs":
+    fp32 [rows, top], the most likely first, the lower id first among equals}."""
+    import torch
+    ctx = _elsewhere(logits.device, stream)
+    if ctx is not None:
+        with ctx:
+            return logprobs(logits, tokens, top)
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.stride(1) != 1:
+        raise ValueError(f"logits: bf16 or fp32 [rows, vocab] with adjacent elements are expected, got {logits.dtype} "
+                         f"{tuple(logits.shape)} with strides {logits.stride()}")
+    rows, vocab = logits.shape
+    dev, n = logits.device, 0
+    if tokens is not None:
+        n = tokens.shape[1] if tokens.dim() == 2 else -1
+        _ints("tokens", tokens, dev, (rows, n))
+    f32 = dict(dtype=torch.float32, device=dev)
+    logp, entropy, best = (torch.empty(s, **f32) for s in ((rows, n), (rows,), (rows, top)))
+    ids = torch.empty((rows, top), dtype=torch.int32, device=dev)
+    check(lib.dflash_logprobs(_ptr(logits), LOGITS_BF16 if logits.dtype == torch.bfloat16 else LOGITS_FP32,
+                              logits.stride(0) if rows > 1 else vocab, rows, vocab, _ptr(tokens), n, top, _ptr(logp),
+                              _ptr(entropy), _ptr(ids), _ptr(best), _stream()))
+    return {"logprobs": logp, "entropy": entropy, "top_ids": ids, "top_logprobs": best}
 
 
 # ----------------------------------------------------------------------------- the verify stack object

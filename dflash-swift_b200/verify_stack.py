@@ -352,11 +352,16 @@ class VerifyStack:
     pre-round state (gated-delta snapshots and conv windows are only read; the new
     states go to `state_out`, the attention caches receive the block's k and v at
     positions context .. context + M - 1), and returns the final-norm hidden states
-    bf16 [M, hidden] (identical on every rank)."""
+    bf16 [M, hidden] (identical on every rank).
+
+    kv_bits (16, 8 or 4): the attention layers run on the batch entries (dflash_batch.h) over
+    a dflashcuda.KVCache of that many bits in groups of kv_group, filled from the bf16 caches
+    of `state`, which the stack then no longer holds; the position is device-resident."""
 
     def __init__(self, cfg: StackConfig, rank: int = 0, world: int = 1, seed: int = 0, device=None,
                  group=None, weights: Optional[dict] = None, state: Optional[dict] = None, allreduce: str = "peer",
-                 tree: bool = False, device_position: bool = False):
+                 tree: bool = False, device_position: bool = False, kv_bits: Optional[int] = None,
+                 kv_group: int = 64):
         import dflashcuda as dc
         self.dc = dc
         self.cfg = cfg
@@ -367,7 +372,8 @@ class VerifyStack:
         # read it from `position` (device int32), which advance() rewrites, so one captured
         # round serves a whole decode loop.
         self.context = cfg.context
-        self.device_position = device_position
+        self.device_position = device_position or kv_bits is not None
+        self.kv_bits = kv_bits
         self.plan = shard_plan(cfg, rank, world)
         self.world = world
         self.pg = group
@@ -376,6 +382,8 @@ class VerifyStack:
             raise RuntimeError("VerifyStack runs on libdflashcuda only (no CPU path)")
         self.w = weights if weights is not None else build_rank_weights(cfg, self.plan, seed, self.device)
         self.state = state if state is not None else build_rank_state(cfg, self.plan, seed, self.device)
+        if kv_bits is not None:
+            self.state = {"layers": [self._batch_state(S, kv_bits, kv_group) for S in self.state["layers"]]}
         self._alloc()
         self.graph = None
         if allreduce not in ("peer", "nccl"):
@@ -387,6 +395,15 @@ class VerifyStack:
         if self.allreduce == "peer":
             self.exchange = self._connect_exchange(rank, self.cfg.hidden)
             self.key_exchange = self._connect_exchange(rank, 4)  # the LM head's argmax keys, 8 bytes a row
+
+    def _batch_state(self, S, bits, group):
+        """A layer's state with its bf16 attention caches replaced by one KVCache of `bits`."""
+        if "cache_k" not in S:
+            return S
+        hkv, max_len, d = S["cache_k"].shape
+        cache = self.dc.KVCache(1, hkv, max_len, d, bits, group, self.device)
+        self.dc.stack_kv_write(cache, S["cache_k"][None], S["cache_v"][None])
+        return {"cache": cache}
 
     def _connect_exchange(self, rank, H):
         """Allocate this rank's exchange buffer for [block, H], swap IPC handles with the
@@ -455,6 +472,11 @@ class VerifyStack:
         d = cfg.head_dim
         self.qkv = torch.empty(M, (2 * p.attn_heads + 2 * p.kv_heads) * d, **bf)
         self.attn_out = torch.empty(M, p.attn_heads * d, **bf)
+        caches = [S["cache"] for S in self.state["layers"] if "cache" in S]
+        if caches:
+            self.attn_q = torch.empty(M, p.attn_heads * d, **bf)
+            self.attn_ws = torch.empty(self.dc.stack_attn_decode_batch_workspace_bytes(caches[0], 0, M, p.attn_heads),
+                                       dtype=torch.uint8, device=dev)
         self.gate_up = torch.empty(M, 2 * p.inter, **bf)
         need = 0
         for L in self.w["layers"]:
@@ -530,12 +552,20 @@ class VerifyStack:
     def _attn(self, L, S):
         cfg, p, dc = self.cfg, self.plan, self.dc
         self._qmm(self.normed, L["qkv"], self.qkv)
+        scale = 1.0 / math.sqrt(cfg.head_dim)
+        if self.kv_bits is not None:
+            width = p.attn_heads * cfg.head_dim
+            parents = None if self.parents is None else self.parents[None]
+            dc.stack_attn_prep_batch(self.qkv, L["q_norm"], L["k_norm"], S["cache"], self.position, p.attn_heads,
+                                     cfg.rotary_dim, cfg.eps, cfg.rope_theta, q_out=self.attn_q, parents=parents)
+            dc.stack_attn_decode_batch(self.attn_q, S["cache"], self.position, scale, out=self.attn_out,
+                                       gate=self.qkv[:, width:2 * width], parents=parents, workspace=self.attn_ws)
+            return self._qmm_reduced(self.attn_out, L["o_proj"])
         dc.stack_attn_prep(self.qkv, L["q_norm"], L["k_norm"], S["cache_k"], S["cache_v"], p.attn_heads, p.kv_heads,
                            cfg.rotary_dim, self.context, cfg.eps, cfg.rope_theta, parents=self.parents,
                            position=self.position)
         dc.stack_attn_decode(self.qkv, S["cache_k"], S["cache_v"], self.attn_out, p.attn_heads, p.kv_heads,
-                             self.context, 1.0 / math.sqrt(cfg.head_dim), parents=self.parents,
-                             position=self.position)
+                             self.context, scale, parents=self.parents, position=self.position)
         return self._qmm_reduced(self.attn_out, L["o_proj"])
 
     def _mlp(self, L):
@@ -592,6 +622,16 @@ class VerifyStack:
         self._forward_body(hidden)
         return self._accept_body(proposals)
 
+    def logprobs(self, tokens=None, top: int = 0):
+        """Log probabilities of the last forward's rows (dflashcuda.logprobs over the LM head's
+        logits): tokens int32 [block, n] on the device, `top` alternatives a row.  One rank only:
+        the ranks of a tensor-parallel stack hold a part of the vocabulary each."""
+        if self.world > 1:
+            raise RuntimeError("logprobs needs the whole vocabulary on one rank (world 1)")
+        q, dc = self.w["lm_head"], self.dc
+        logits = dc.qmm(self.out, q.w, q.scales, q.biases, q.group, q.bits, workspace=self.ws)
+        return dc.logprobs(logits, tokens, top)
+
     def set_tree(self, parents):
         """The next rounds verify a speculative tree: parents[r] is row r's parent row (-1
         for the anchor row 0), cfg.block rows.  Call between rounds, never while a round is
@@ -644,6 +684,7 @@ class VerifyStack:
         if self.tree_plan is None and rows != list(range(keep)):
             raise ValueError(f"a chain round keeps rows 0 .. keep-1, not {rows}")
         C = (2 * (p.gdn_key_heads or p.gdn_heads) + p.gdn_heads) * cfg.gdn_dk
+        moved = count = None
         gi = 0
         for L, S in zip(self.w["layers"], self.state["layers"]):
             if L["kind"] == "gdn":
@@ -657,11 +698,19 @@ class VerifyStack:
                 S["window"].copy_(window)
                 gi += 1
             elif rows != list(range(keep)):
-                dc.stack_kv_compact(S["cache_k"], S["cache_v"], self.context, rows)
+                if self.kv_bits is not None:
+                    if moved is None:
+                        moved = torch.tensor([rows], dtype=torch.int32, device=self.device)
+                        count = torch.tensor([keep], dtype=torch.int32, device=self.device)
+                    dc.stack_kv_compact_batch(S["cache"], self.position, moved, count)
+                else:
+                    dc.stack_kv_compact(S["cache_k"], S["cache_v"], self.context, rows)
 
     def advance(self, n: int):
         """After commit(rows): the caches now hold n = len(rows) more tokens."""
-        if n < 0 or any(S["cache_k"].shape[1] < self.context + n for S in self.state["layers"] if "cache_k" in S):
+        ends = [S["cache"].max_len if "cache" in S else S["cache_k"].shape[1] for S in self.state["layers"]
+                if "cache" in S or "cache_k" in S]
+        if n < 0 or any(end < self.context + n for end in ends):
             raise ValueError(f"advancing the context by {n} runs past the attention caches")
         self.context += n
         if self.position is not None:  # stream-ordered after the round that was just read back
@@ -703,6 +752,7 @@ PHASES = {
     "stack_gdn_conv_gates": "gated-delta conv + gates", "gdn_step": "gated-delta step",
     "gdn_step_tree": "gated-delta step", "stack_gated_norm": "gated norm",
     "stack_attn_prep": "attention prep", "stack_attn_decode": "decode attention",
+    "stack_attn_prep_batch": "attention prep", "stack_attn_decode_batch": "decode attention",
 }
 
 
@@ -779,6 +829,9 @@ def main(argv=None) -> int:
                     help="gated-delta q / k heads, each shared by gdn_heads / this many value heads")
     ap.add_argument("--phase-times", action="store_true",
                     help="also report one eager forward's device time split by the role of each library call")
+    ap.add_argument("--kv-bits", type=int, choices=[16, 8, 4], default=None,
+                    help="attention caches of this many bits, on the batch entries (default: the bf16 single-sequence "
+                         "entries)")
     ap.add_argument("--tree", default=None,
                     help="verify a speculative tree instead of a chain: comma-separated parent rows, one per "
                          "block row (-1 for the anchor), e.g. -1,0,0,1,1,2,3,5")
@@ -802,7 +855,7 @@ def main(argv=None) -> int:
         cfg = replace(cfg, gdn_key_heads=args.gdn_key_heads)
 
     stack = VerifyStack(cfg, rank, world, seed=args.seed, device=dev, group=pg, allreduce=args.allreduce,
-                        tree=args.tree is not None)
+                        tree=args.tree is not None, kv_bits=args.kv_bits)
     if args.tree is not None:
         stack.set_tree([int(v) for v in args.tree.split(",")])
     hidden = make_block(cfg, args.seed, dev)
