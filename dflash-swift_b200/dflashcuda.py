@@ -39,6 +39,7 @@ DEVERR_QMM_PIPELINE = 0x1
 DEVERR_QMM_REDUCE = 0x2
 DEVERR_ALLREDUCE = 0x4
 DEVERR_POSITION = 0x8
+DEVERR_ATTN_PIPELINE = 0x10
 DEVERR_TEST_WAIT = 0x80000000
 
 # Every symbol the header declares; tests check the library exports all of them.
