@@ -21,11 +21,13 @@
 //
 // Roles: warps 0-7 softmax (two per TMEM lane quarter, half of the columns each), 8-15 producers
 // (cache rows to swizzled shared memory boxes of 128 keys x 64 elements, in a ring), warp 16 issues
-// the products.  The running maximum is only raised when a score passes it by kLazy (in powers
+// the products (17-19 have no work).  The running maximum is only raised when a score passes it by kLazy (in powers
 // of two), so the accumulators are rarely rescaled.
 #include "common.cuh"
 #include "dflash_batch.h"
 #include "tcgen05.cuh"
+
+#include <cstddef>
 
 namespace dflash {
 namespace attn {
@@ -34,16 +36,53 @@ constexpr int kKeys = 128;
 constexpr int kRows = 128;
 constexpr int kBox = kKeys * 128;          // bytes of a ring slot: 128 keys x 64 elements of 16 bits
 constexpr int kSoftmaxWarps = 8, kProducerWarps = 8;
-constexpr int kThreads = 32 * (kSoftmaxWarps + kProducerWarps + 1);
+constexpr int kThreads = 32 * (kSoftmaxWarps + kProducerWarps + 4);  // whole warpgroups: registers move between them
+// Registers a thread.  The block starts with kThreads x 96 = 61440 and every warpgroup takes or gives; what is
+// taken is never more than what is given, so nobody waits for good:
+//   quantised: 256 x 96 + 256 x 120 + 128 x 40 = 60416 (the producers hold two tiles of codes),
+//   bf16:     256 x 120 + 256 x 72 + 128 x 40 = 54272.
+constexpr int kIssueRegs = 40;
 constexpr int kMaxCtas = 160;              // partials are sized for this many CTAs
 constexpr int kMaxSlots = 10;
 constexpr int kScaleDepth = 4;             // tiles whose key factors may be alive at once
 constexpr int kPoison = 16;                // units whose poison flags may be alive at once
 constexpr float kLazy = 4.f;               // a maximum moves when a score passes it by 2^4 ...
 constexpr float kLift = 8.f;               // ... and P is 2^8 p, up to 2^12: small weights stay normal in fp16
-constexpr int kTop = 12;                   // fp16 operands are scaled to 2^12 .. 2^13
+constexpr int kTopQ = 12;                  // query rows are scaled to 2^12 .. 2^13 in fp16
 constexpr uint32_t kTmemColumns = 512;
-constexpr int kSmemLimit = 232448 - 1024;
+constexpr int kSmemLimit = 232448;
+
+// Shared memory: what has a fixed size first, so that its addresses are constants; then the scale
+// tables, and from the next 1024-byte border on the ring, Q and P.
+struct Fixed {
+    uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full, pv_done, q_full, sc_full[kScaleDepth],
+        sc_empty[kScaleDepth];
+    alignas(16) float thr[kRows];       // read four at a time, like mm and qs
+    float mm[kRows], qs[kRows], corr[kRows], m[kRows];
+    int info[kRows];                    // chain: the row's token; tree: its path mask
+    float part[4][kRows];
+    float key_k[kScaleDepth][kKeys], key_v[kScaleDepth][kKeys];
+    uint16_t key_w[kScaleDepth][kKeys];
+    int poison[kPoison];
+    int abort, tmem, w0, w1, entry, off;
+    int unit_tiles, unit_rows;          // for the issuing thread, from the softmax warps
+    int warp_sum[kThreads / 32];
+};
+static_assert(offsetof(Fixed, thr) % 16 == 0 && offsetof(Fixed, mm) % 16 == 0 && offsetof(Fixed, qs) % 16 == 0 &&
+                  offsetof(Fixed, key_w) % 4 == 0 && alignof(Fixed) == 16, "vector accesses");
+constexpr uint32_t kTables = (sizeof(Fixed) + 15) / 16 * 16;
+
+struct Layout {
+    uint32_t ring, q, p, total;
+};
+__host__ inline Layout layout(int d, int nr, int slots, int groups) {
+    Layout l;
+    l.ring = (kTables + 3 * kKeys * groups * 4 + 1023) / 1024 * 1024;
+    l.q = l.ring + slots * kBox;
+    l.p = l.q + nr * d * 2;
+    l.total = l.p + kKeys * nr * 2;
+    return l;
+}
 
 struct Args {
     const uint16_t* q;
@@ -60,6 +99,7 @@ struct Args {
     int rows_o;                  // rows of a block of one sequence, at most
     int nr;                      // columns of the products' buffers: 64 or kRows
     int slots;                   // ring slots
+    Layout l;
     // workspace: partials of the prefix, then of the sequences
     int32_t* first;              // [segments] first and last CTA of each (row block, kv head)
     int32_t* last;
@@ -82,28 +122,6 @@ __device__ __forceinline__ long long partial_row(const Args& a, bool prefix, lon
 }
 __device__ __forceinline__ long long partial_index(const Args& a, bool prefix, long long segment, int cta) {
     return prefix ? segment + cta : partials_p(a) + segment + cta;
-}
-
-// Shared memory behind the ring, Q and P: offsets in bytes.
-struct Layout {
-    uint32_t q, p, scale_k, scale_v, key_k, key_v, key_w, row, part, bars, misc, total;
-};
-__host__ __device__ inline Layout layout(int d, int nr, int slots, int groups) {
-    Layout l;
-    uint32_t at = slots * kBox;
-    l.q = at;             at += nr * d * 2;
-    l.p = at;             at += kKeys * nr * 2;
-    l.scale_k = at;       at += kKeys * groups * 4;
-    l.scale_v = at;       at += 2 * kKeys * groups * 4;
-    l.key_k = at;         at += groups ? kScaleDepth * kKeys * 4 : 0;
-    l.key_v = at;         at += groups ? kScaleDepth * kKeys * 4 : 0;
-    l.key_w = at;         at += groups ? kScaleDepth * kKeys * 2 : 0;
-    l.row = at;           at += 6 * kRows * 4;
-    l.part = at;          at += 4 * kRows * 4;
-    l.bars = at;          at += 8 * (2 * kMaxSlots + 2 + 1 + 1 + 1 + 2 * kScaleDepth + 1);
-    l.misc = at;          at += 4 * (kPoison + 8 + 40);
-    l.total = at;
-    return l;
 }
 
 // ---------------------------------------------------------------- units of a CTA's run
@@ -196,9 +214,9 @@ __device__ __forceinline__ uint32_t fma_h2(uint32_t a, uint32_t b, uint32_t c) {
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
-__device__ __forceinline__ uint32_t sub_h2(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
     uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
@@ -236,60 +254,52 @@ __device__ __forceinline__ int order(int i) {
     return BITS == 4 ? (i >> 1) + 4 * (i & 1) : i;
 }
 
+__device__ __forceinline__ bool try_wait_1us(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // ---------------------------------------------------------------- the kernel
 template <int BITS, int D>
 struct Kernel {
     static constexpr bool kQuant = BITS != 16;
+    // Keys are scaled to 2^kTop .. 2^(kTop + 1): the step of a group, at most 2^(kTop + 2) / (2^BITS - 1), has
+    // to stay under 2^-8 (store_groups).
+    static constexpr int kTop = BITS == 8 ? -3 : -7;
     static constexpr int NB = D / 64;                  // boxes of a K or V tile
     static constexpr int MB = D > 64 ? D / 128 : 1;    // 128-lane blocks of O^T (half used when d is 64)
-    static constexpr int kLoads = kQuant ? NB * BITS / 4 : 1;  // 16-byte loads of codes a producer thread makes per tile
+    static constexpr int kLoads = kQuant ? NB * BITS / 4 : 1;  // 16-byte loads of codes a producer thread makes per K or V tile
 
-    struct Shared {
-        uint32_t base;  // shared address of the ring
-        Layout l;
-        uint64_t *full, *empty, *s_full, *p_full, *pv_done, *q_full, *sc_full, *sc_empty;
-        int* poison;
-        int* misc;  // 0 abort, 1 tmem, 2 run start, 3 run end, 4 entry, 5 off
-        volatile int* abort;
-        float *thr, *mm, *qs, *corr, *m;
-        int* rowinfo;  // chain: the row's token; tree: its path mask
-        float* part;
-    };
+    __device__ static __forceinline__ Fixed& fixed() {
+        extern __shared__ __align__(1024) uint8_t smem[];
+        return *reinterpret_cast<Fixed*>(smem);
+    }
+    __device__ static __forceinline__ uint32_t smem_at(uint32_t offset) { return smem_u32(&fixed()) + offset; }
 
-    __device__ static __forceinline__ void wait(const Shared& s, uint64_t* bar, uint32_t parity) {
-        mbar_wait_bounded(bar, parity, s.abort, DFLASH_DEVERR_ATTN_PIPELINE);
+    // A bounded wait that stays small where it is inlined: a failed try sleeps up to a microsecond, and
+    // 2^20 of them (a second at most) raise the error.  No clock is read, whose read costs more than the
+    // usual wait.  After an error every wait returns at once and the roles run on to their ends.
+    __device__ static __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
+        if (mbar_try_wait(bar, parity)) return;
+        for (int n = 0; !try_wait_1us(bar, parity); ++n) {
+            if (*const_cast<volatile int*>(&fixed().abort)) return;
+            if (n == 1 << 20) {
+                atomicOr(&g_device_error, DFLASH_DEVERR_ATTN_PIPELINE);
+                *const_cast<volatile int*>(&fixed().abort) = 1;
+            }
+        }
     }
 
     // ------------------------------------------------------------ producers
-    struct Tile {            // where a tile's rows lie
-        const kv::View* c;
-        int64_t row0;
-        int valid;           // rows that exist and that some query row sees
-        int suspect;         // rows from here on are hidden from some query row
-        int poison;          // flag of the unit
-    };
-    struct TileWalk {
-        Walker w;
-        Unit u;
-        int i, unit;
-        __device__ __forceinline__ bool next(const Args& a, Tile& t, bool& first) {
-            first = false;
-            if (i == u.n) {
-                if (!w.next(a, u)) return false;
-                i = 0;
-                ++unit;
-                first = true;
-            }
-            const int tile = u.t0 + i++;
-            t.c = u.prefix ? &a.prefix : &a.cache;
-            t.row0 = kv::row_index(*t.c, u.seq, u.head, tile * kKeys);
-            t.valid = min(kKeys, u.keys - tile * kKeys);
-            t.suspect = u.prefix ? kKeys : max(0, u.len - tile * kKeys);
-            t.poison = unit & (kPoison - 1);
-            return true;
-        }
-    };
-
+    // Boxes are produced in the order in which the products take them: in each unit K(0), then K(i)
+    // V(i - 1), then V(n - 1).
     struct Ring {
         int slot;
         uint32_t phase;
@@ -301,59 +311,74 @@ struct Kernel {
         }
     };
 
-    // A non-finite element of a row that some query row does not see would reach it as 0 * inf: it
-    // is taken out of the operand and the unit's flag raised, for the join to put it back where it
-    // is seen.  v holds eight 16-bit elements.
-    __device__ static __forceinline__ void clean(uint4& v, int* flag) {
-        constexpr uint32_t kExp = kQuant ? 0x7c00u : 0x7f80u;
-        uint32_t* w = &v.x;
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if ((w[i] & kExp) == kExp) { w[i] &= 0xffff0000u; bad = true; }
-            if ((w[i] & (kExp << 16)) == (kExp << 16)) { w[i] &= 0x0000ffffu; bad = true; }
+    // Where the rows of a unit's (sequence, kv head) lie.
+    struct Source {
+        const uint8_t *k, *v;
+        int64_t row0;
+        bool prefix;
+        int keys;    // rows that exist and that some query row sees
+        int hidden;  // rows from here on are hidden from some query row
+        int t0, n;
+        __device__ __forceinline__ Source() {}
+        __device__ __forceinline__ Source(const Args& a, const Unit& u) {
+            const kv::View& c = u.prefix ? a.prefix : a.cache;
+            row0 = kv::row_index(c, u.seq, u.head, 0);
+            k = c.k + row0 * (D * BITS / 8);
+            v = c.v + row0 * (D * BITS / 8);
+            prefix = u.prefix;
+            keys = u.keys;
+            hidden = u.prefix ? u.keys : u.len;
+            t0 = u.t0;
+            n = u.n;
         }
-        if (bad) *flag = 1;
-    }
+    };
 
-    __device__ static __forceinline__ void signal_full(const Shared& s, int slot) {
+    __device__ static __forceinline__ void signal_full(int slot) {
         fence_proxy_async_shared();
         __syncwarp();
-        if ((threadIdx.x & 31) == 0) mbar_arrive(&s.full[slot]);
+        if ((threadIdx.x & 31) == 0) mbar_arrive(&fixed().full[slot]);
+    }
+
+    // The pieces of a box that a producer thread writes: kPieces rows, kChunks 16-byte chunks of each.
+    static constexpr int kPieces = kQuant ? BITS / 4 : 4, kChunks = kQuant ? 16 / BITS : 1;
+    static constexpr int kRowThreads = kQuant ? BITS / 2 : 8;  // threads that share a row
+    __device__ static __forceinline__ int piece_key(int pt, int u) { return pt / kRowThreads + u * (256 / kRowThreads); }
+
+    // A non-finite element of a row that some query row does not see would reach it as 0 * inf: it is
+    // taken out of the operand and the unit's flag raised, for the join to put it back where it is
+    // seen.  Each thread looks at what it wrote itself.
+    __device__ static __forceinline__ void take_out(uint32_t box, int from, int pt, int* flag) {
+        constexpr uint32_t kExp = kQuant ? 0x7c00u : 0x7f80u;
+#pragma unroll 1
+        for (int u = 0; u < kPieces * kChunks; ++u) {
+            const int key = piece_key(pt, u / kChunks), chunk = (pt % kRowThreads) * kChunks + u % kChunks;
+            if (key < from) continue;
+            const uint32_t addr = box + key * 128 + ((chunk ^ (key & 7)) << 4);
+            const uint4 x = lds128(addr);
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if ((w[i] & kExp) == kExp) { w[i] &= 0xffff0000u; bad = true; }
+                if ((w[i] & (kExp << 16)) == (kExp << 16)) { w[i] &= 0x0000ffffu; bad = true; }
+            }
+            if (bad) {
+                sts128(addr, make_uint4(w[0], w[1], w[2], w[3]));
+                *reinterpret_cast<volatile int*>(flag) = 1;
+            }
+        }
     }
 
     // bf16 caches: cp.async straight into the swizzled boxes, up to kLag boxes in flight.
     static constexpr int kLag = 5;
 
-    __device__ static void produce_bf16(const Args& a, const Shared& s, Walker w0) {
-        const int pt = threadIdx.x - 32 * kSoftmaxWarps;
+    __device__ static void produce_bf16(const Args& a, Walker w) {
+        const int pt = threadIdx.x - 32 * kSoftmaxWarps, key0 = pt >> 3, c = pt & 7;
+        const uint32_t ring_at = smem_at(a.l.ring), dst0 = ring_at + key0 * 128 + ((c ^ (key0 & 7)) << 4);
         Ring ring{0, 0};
         int done_slot = 0, pending = 0;
-        // what to look at in the boxes in flight (a queue of kLag)
-        int q_from[kLag] = {}, q_flag[kLag] = {};
-        const auto retire = [&]() {  // the oldest box in flight is complete
-            if (q_from[0] < kKeys) {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int key = (pt + 256 * u) >> 3, c = pt & 7;
-                    if (key >= q_from[0]) {
-                        const uint32_t addr = s.base + done_slot * kBox + key * 128 + ((c ^ (key & 7)) << 4);
-                        uint4 v = lds128(addr);
-                        clean(v, &s.poison[q_flag[0]]);
-                        sts128(addr, v);
-                    }
-                }
-            }
-            signal_full(s, done_slot);
-            if (++done_slot == a.slots) done_slot = 0;
-#pragma unroll
-            for (int i = 0; i + 1 < kLag; ++i) {
-                q_from[i] = q_from[i + 1];
-                q_flag[i] = q_flag[i + 1];
-            }
-            --pending;
-        };
-        const auto wait_oldest = [&]() {
+        int from[kLag] = {}, flag[kLag] = {};  // what to look at in the boxes in flight, oldest first
+        const auto retire_oldest = [&]() {
             switch (pending) {
                 case 1: cp_async_wait<0>(); break;
                 case 2: cp_async_wait<1>(); break;
@@ -361,73 +386,80 @@ struct Kernel {
                 case 4: cp_async_wait<3>(); break;
                 default: cp_async_wait<4>(); break;
             }
-            retire();
-        };
-        const auto box = [&](const Tile& t, bool is_v, int b) {
-            if (pending == kLag) wait_oldest();
-            const uint32_t parity = ring.phase ^ 1;
-            while (pending > 0 && !mbar_try_wait(&s.empty[ring.slot], parity)) wait_oldest();
-            wait(s, &s.empty[ring.slot], parity);
-            const uint16_t* src = reinterpret_cast<const uint16_t*>(is_v ? t.c->v : t.c->k);
+            if (__builtin_expect(from[0] < kKeys, 0)) take_out(ring_at + done_slot * kBox, from[0], pt, &fixed().poison[flag[0]]);
+            signal_full(done_slot);
+            if (++done_slot == a.slots) done_slot = 0;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int key = (pt + 256 * u) >> 3, c = pt & 7;
-                const bool live = key < t.valid;
-                cp_async16(s.base + ring.slot * kBox + key * 128 + ((c ^ (key & 7)) << 4),
-                           src + (t.row0 + (live ? key : 0)) * D + b * 64 + c * 8, live);
+            for (int i = 0; i + 1 < kLag; ++i) {
+                from[i] = from[i + 1];
+                flag[i] = flag[i + 1];
             }
-            cp_async_commit();
+            --pending;
+        };
+        Unit u;
+        for (int unit = 0; w.next(a, u); ++unit) {
+            const Source src(a, u);
+#pragma unroll 1
+            for (int step = 1; step <= 2 * src.n; ++step) {  // K0 K1 V0 K2 V1 .. V(n-1)
+                const bool is_v = step > 1 && (step == 2 * src.n || (step & 1));
+                const int i = is_v ? (step == 2 * src.n ? src.n - 1 : step / 2 - 1) : step / 2;
+                const int key_at = (src.t0 + i) * kKeys, valid = min(kKeys, src.keys - key_at);
+                const int look = max(0, src.hidden - key_at);
+                const uint8_t* p = (is_v ? src.v : src.k) + ((int64_t)(key_at + key0) * D + c * 8) * 2;
+#pragma unroll 1
+                for (int b = 0; b < NB; ++b, p += 128) {
+                    if (pending == kLag) retire_oldest();
+                    while (!mbar_try_wait(&fixed().empty[ring.slot], ring.phase ^ 1)) {
+                        if (pending == 0) {
+                            wait(&fixed().empty[ring.slot], ring.phase ^ 1);
+                            break;
+                        }
+                        retire_oldest();
+                    }
 #pragma unroll
-            for (int i = 0; i < kLag; ++i)
-                if (i == pending) {
-                    q_from[i] = is_v && t.suspect < t.valid ? t.suspect : kKeys;
-                    q_flag[i] = t.poison;
+                    for (int x = 0; x < 4; ++x) {
+                        const bool live = key0 + 32 * x < valid;
+                        cp_async16(dst0 + ring.slot * kBox + x * 4096, live ? p + x * (32 * D * 2) : src.k, live);
+                    }
+                    cp_async_commit();
+#pragma unroll
+                    for (int x = 0; x < kLag; ++x)
+                        if (x == pending) {
+                            from[x] = is_v && look < valid ? look : kKeys;
+                            flag[x] = unit & (kPoison - 1);
+                        }
+                    ++pending;
+                    ring.step(a.slots);
                 }
-            ++pending;
-            ring.step(a.slots);
-        };
-        TileWalk tw{w0, Unit{}, 0, -1};
-        tw.u.n = 0;
-        Tile t, prev;
-        bool first, have_prev = false;
-        while (tw.next(a, t, first)) {
-            if (first && have_prev) {  // the unit before ends with its last V
-                for (int b = 0; b < NB; ++b) box(prev, true, b);
-                have_prev = false;
             }
-            for (int b = 0; b < NB; ++b) box(t, false, b);
-            if (have_prev)
-                for (int b = 0; b < NB; ++b) box(prev, true, b);
-            prev = t;
-            have_prev = true;
         }
-        if (have_prev)
-            for (int b = 0; b < NB; ++b) box(prev, true, b);
-        while (pending > 0) wait_oldest();
+        while (pending > 0) retire_oldest();
     }
 
     // Quantised caches: codes to registers a tile ahead, unpacked to fp16 and stored swizzled.
-    __device__ static __forceinline__ void load_codes(const Tile& t, bool is_v, int pt, uint4 (&r)[kLoads]) {
-        const uint8_t* src = (is_v ? t.c->v : t.c->k) + t.row0 * (D * BITS / 8);
-        constexpr int kPer = BITS / 2;  // 16-byte pieces of a key in a box
+    __device__ static __forceinline__ void load_codes(const uint8_t* rows, int tile, int keys, int pt, uint4 (&r)[kLoads]) {
+        const int valid = keys - tile * kKeys;
+        const uint8_t* p = rows + (int64_t)(tile * kKeys + pt / kRowThreads) * (D * BITS / 8) + (pt % kRowThreads) * 16;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int box = i / (BITS / 4), idx = pt + 256 * (i % (BITS / 4)), key = idx / kPer, piece = idx % kPer;
-            r[i] = key < t.valid ? __ldcs(reinterpret_cast<const uint4*>(src + (size_t)key * (D * BITS / 8) + box * (8 * BITS) +
-                                                                         piece * 16))
-                                 : make_uint4(0, 0, 0, 0);
+            const int b = i / kPieces, u = i % kPieces;
+            r[i] = piece_key(pt, u) < valid ? __ldcs(reinterpret_cast<const uint4*>(
+                                                  p + b * (8 * BITS) + u * (256 / kRowThreads) * (D * BITS / 8)))
+                                            : make_uint4(0, 0, 0, 0);
         }
     }
     // Scales and biases of one key, as raw bf16 pairs.
     struct Groups {
         uint32_t s[4], b[4];
     };
-    __device__ static __forceinline__ void load_groups(const Tile& t, bool is_v, int key, int groups, Groups& g) {
-        const uint16_t* ps = (is_v ? t.c->vs : t.c->ks) + (t.row0 + key) * groups;
-        const uint16_t* pb = (is_v ? t.c->vb : t.c->kb) + (t.row0 + key) * groups;
+    __device__ static __forceinline__ void load_groups(const Args& a, const Source& src, bool is_v, int key, int groups,
+                                                       Groups& g) {
+        const kv::View& c = src.prefix ? a.prefix : a.cache;
+        const int64_t at = (src.row0 + key) * groups;
+        const uint16_t *ps = (is_v ? c.vs : c.ks) + at, *pb = (is_v ? c.vb : c.kb) + at;
 #pragma unroll
         for (int i = 0; i < 4; ++i) g.s[i] = g.b[i] = 0;
-        if (key >= t.valid) return;
+        if (key >= src.keys) return;
         if (groups == 1) {
             g.s[0] = *ps;
             g.b[0] = *pb;
@@ -445,189 +477,193 @@ struct Kernel {
         constexpr float kCodes = BITS == 8 ? 255.f : 15.f;
         float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < groups) {
-                const float sc = __uint_as_float(i & 1 ? g.s[i / 2] & 0xffff0000u : g.s[i / 2] << 16);
-                const float bi = __uint_as_float(i & 1 ? g.b[i / 2] & 0xffff0000u : g.b[i / 2] << 16);
-                m = fmaxf(m, fmaxf(fabsf(bi), fabsf(fmaf(kCodes, sc, bi))));
+        for (int i = 0; i < 4; ++i)
+            if (2 * i < groups) {
+                const float s0 = __uint_as_float(g.s[i] << 16), s1 = __uint_as_float(g.s[i] & 0xffff0000u);
+                const float b0 = __uint_as_float(g.b[i] << 16), b1 = __uint_as_float(g.b[i] & 0xffff0000u);
+                m = fmaxf(m, fmaxf(fabsf(b0), fabsf(fmaf(kCodes, s0, b0))));
+                m = fmaxf(m, fmaxf(fabsf(b1), fabsf(fmaf(kCodes, s1, b1))));  // zero where groups is 1
             }
         return m;
     }
+    // Table entries (fp16 scale * f * 2^24, bias * f): a code in the low bits of a half is the subnormal
+    // code * 2^-24, so that one fma gives scale * code + bias (|scale * f| < 2^-8: see kTop).
     __device__ static __forceinline__ void store_groups(uint32_t addr, const Groups& g, int groups, float f) {
+        const float f24 = f * 16777216.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < groups) {
-                const float sc = __uint_as_float(i & 1 ? g.s[i / 2] & 0xffff0000u : g.s[i / 2] << 16);
-                const float bi = __uint_as_float(i & 1 ? g.b[i / 2] & 0xffff0000u : g.b[i / 2] << 16);
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr + 4 * i), "r"(pack2<false>(sc * f, bi * f)) : "memory");
+        for (int i = 0; i < 4; ++i)
+            if (2 * i < groups) {
+                const uint32_t e0 = pack2<false>(__uint_as_float(g.s[i] << 16) * f24, __uint_as_float(g.b[i] << 16) * f);
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr + 8 * i), "r"(e0) : "memory");
+                if (groups > 1) {
+                    const uint32_t e1 = pack2<false>(__uint_as_float(g.s[i] & 0xffff0000u) * f24,
+                                                     __uint_as_float(g.b[i] & 0xffff0000u) * f);
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr + 8 * i + 4), "r"(e1) : "memory");
+                }
             }
     }
-    // Unpacks one 16-byte piece (32 or 16 elements of one key and group) into its 16-byte chunks of a box.
-    __device__ static __forceinline__ void unpack(uint4 codes, uint32_t sb, uint32_t row_addr, int key, int piece, bool suspect,
-                                                  int* flag) {
+    // Unpacks one 16-byte piece (32 or 16 elements of one key and group) into its chunks of a box row.
+    __device__ static __forceinline__ void unpack(uint4 codes, uint32_t sb, uint32_t row, int key, int piece) {
         const uint32_t s2 = __byte_perm(sb, 0, 0x1010), b2 = __byte_perm(sb, 0, 0x3232);
         const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-        constexpr uint32_t kMagic = 0x64006400u;  // fp16 1024 + code
         if constexpr (BITS == 4) {
+            const uint32_t t2 = mul_h2(s2, 0x2c002c00u);  // 2^-4: codes four bits further up
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                uint4 v;
-                uint32_t* p = &v.x;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    p[j] = fma_h2(sub_h2((w[i] >> (4 * j)) & 0x000f000fu | kMagic, kMagic), s2, b2);
-                if (suspect) clean(v, flag);
-                sts128(row_addr + (((4 * piece + i) ^ (key & 7)) << 4), v);
+                const uint32_t hi = w[i] >> 8;
+                sts128(row + (((4 * piece + i) ^ (key & 7)) << 4),
+                       make_uint4(fma_h2(w[i] & 0x000f000fu, s2, b2), fma_h2(w[i] & 0x00f000f0u, t2, b2),
+                                  fma_h2(hi & 0x000f000fu, s2, b2), fma_h2(hi & 0x00f000f0u, t2, b2)));
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint4 v;
-                v.x = fma_h2(sub_h2(__byte_perm(w[2 * i], kMagic, 0x5150), kMagic), s2, b2);
-                v.y = fma_h2(sub_h2(__byte_perm(w[2 * i], kMagic, 0x5352), kMagic), s2, b2);
-                v.z = fma_h2(sub_h2(__byte_perm(w[2 * i + 1], kMagic, 0x5150), kMagic), s2, b2);
-                v.w = fma_h2(sub_h2(__byte_perm(w[2 * i + 1], kMagic, 0x5352), kMagic), s2, b2);
-                if (suspect) clean(v, flag);
-                sts128(row_addr + (((2 * piece + i) ^ (key & 7)) << 4), v);
-            }
+            for (int i = 0; i < 2; ++i)
+                sts128(row + (((2 * piece + i) ^ (key & 7)) << 4),
+                       make_uint4(fma_h2(__byte_perm(w[2 * i], 0, 0x4140), s2, b2),
+                                  fma_h2(__byte_perm(w[2 * i], 0, 0x4342), s2, b2),
+                                  fma_h2(__byte_perm(w[2 * i + 1], 0, 0x4140), s2, b2),
+                                  fma_h2(__byte_perm(w[2 * i + 1], 0, 0x4342), s2, b2)));
         }
     }
 
-    __device__ static void produce_quant(const Args& a, const Shared& s, Walker w0) {
+    __device__ static void produce_quant(const Args& a, Walker w) {
         const int pt = threadIdx.x - 32 * kSoftmaxWarps, groups = D / a.cache.group;
-        const int key_of = pt & (kKeys - 1);
+        const int key_of = pt & (kKeys - 1), piece = pt % kRowThreads;
         const bool does_v = pt >= kKeys;
+        const uint32_t v_bytes = kKeys * groups * 4, tk = smem_at(kTables), tv = tk + v_bytes;
+        const uint32_t ring_at = smem_at(a.l.ring);
+        const int shift = 31 - __clz(a.cache.group);
         Ring ring{0, 0};
-        const auto emit = [&](const Tile& t, bool is_v, const uint4 (&r)[kLoads], uint32_t table) {
+        // look: first row of the tile to look at for non-finite values, kKeys for none
+        const auto emit = [&](const uint4 (&r)[kLoads], uint32_t table, int look, int unit) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                wait(s, &s.empty[ring.slot], ring.phase ^ 1);
-                const uint32_t box = s.base + ring.slot * kBox;
-                constexpr int kPer = BITS / 2;
+                wait(&fixed().empty[ring.slot], ring.phase ^ 1);
+                const uint32_t box = ring_at + ring.slot * kBox;
 #pragma unroll
-                for (int u = 0; u < BITS / 4; ++u) {
-                    const int idx = pt + 256 * u, key = idx / kPer, piece = idx % kPer;
-                    const int element = b * 64 + piece * (128 / BITS);
-                    const uint32_t sb = lds32(table + (key * groups + element / a.cache.group) * 4);
-                    unpack(r[b * (BITS / 4) + u], sb, box + key * 128, key, piece, is_v && key >= t.suspect && key < t.valid,
-                           &s.poison[t.poison]);
+                for (int u = 0; u < kPieces; ++u) {
+                    const int key = piece_key(pt, u), group = (b * 64 + piece * (128 / BITS)) >> shift;
+                    unpack(r[b * kPieces + u], lds32(table + (key * groups + group) * 4), box + key * 128, key, piece);
                 }
-                signal_full(s, ring.slot);
+                if (__builtin_expect(look < kKeys, 0)) take_out(box, look, pt, &fixed().poison[unit & (kPoison - 1)]);
+                signal_full(ring.slot);
                 ring.step(a.slots);
             }
         };
-        TileWalk tw{w0, Unit{}, 0, -1};
-        tw.u.n = 0;
-        Tile t, next, prev;
-        bool first, next_first = false, more;
+        Unit u;
+        if (!w.next(a, u)) return;
+        Source cur(a, u), next;
         uint4 kr[kLoads], vr[kLoads];
         Groups g;
-        if (!tw.next(a, t, first)) return;
-        load_codes(t, false, pt, kr);
-        load_groups(t, does_v, key_of, groups, g);
-        const uint32_t tk = s.base + s.l.scale_k, tv = s.base + s.l.scale_v, v_bytes = kKeys * groups * 4;
-        bool have_prev = false;
-        for (int i = 0;; ++i) {
-            if (first && have_prev) {
-                emit(prev, true, vr, tv + ((i - 1) & 1) * v_bytes);
-                have_prev = false;
+        load_codes(cur.k, cur.t0, cur.keys, pt, kr);
+        load_groups(a, cur, does_v, cur.t0 * kKeys + key_of, groups, g);
+        int tile = 0;
+        bool more = true;
+        for (int unit = 0; more; ++unit) {
+            more = w.next(a, u);
+            if (more) next = Source(a, u);
+#pragma unroll 1
+            for (int i = 0; i <= cur.n; ++i, ++tile) {
+                if (i < cur.n) {
+                    // key factors of this tile: K's by the lower 128 threads, V's by the upper ones
+                    const int depth = tile % kScaleDepth;
+                    wait(&fixed().sc_empty[depth], ((tile / kScaleDepth) & 1) ^ 1);
+                    named_bar_sync(3, 32 * kProducerWarps);  // every thread is done with the tables that are rewritten
+                    const float top = largest(g, groups);
+                    if (does_v) {
+                        const int e = min(max(exponent(top), -15), 24);
+                        store_groups(tv + (tile & 1) * v_bytes + key_of * groups * 4, g, groups, exp2i(kTop - e));
+                        fixed().key_v[depth][key_of] = e;
+                        fixed().key_w[depth][key_of] = static_cast<uint16_t>(pack2<false>(exp2i(-e), 0.f));
+                    } else {
+                        const int e = min(max(exponent(top), -100), 120);
+                        store_groups(tk + key_of * groups * 4, g, groups, exp2i(kTop - e));
+                        fixed().key_k[depth][key_of] = exp2i(e - kTop);
+                    }
+                    named_bar_sync(3, 32 * kProducerWarps);
+                    if (pt == 0) mbar_arrive(&fixed().sc_full[depth]);
+                    const bool last = i + 1 == cur.n;
+                    if (!last) load_groups(a, cur, does_v, (cur.t0 + i + 1) * kKeys + key_of, groups, g);
+                    else if (more) load_groups(a, next, does_v, next.t0 * kKeys + key_of, groups, g);
+                    emit(kr, tk, kKeys, 0);
+                    if (!last) load_codes(cur.k, cur.t0 + i + 1, cur.keys, pt, kr);
+                    else if (more) load_codes(next.k, next.t0, next.keys, pt, kr);
+                }
+                if (i > 0) {
+                    const int at = (cur.t0 + i - 1) * kKeys, look = max(0, cur.hidden - at);
+                    emit(vr, tv + ((tile - 1) & 1) * v_bytes, at + look < cur.keys ? look : kKeys, unit);
+                }
+                if (i < cur.n) load_codes(cur.v, cur.t0 + i, cur.keys, pt, vr);
             }
-            // key factors of this tile: K by the lower 128 threads, V by the upper ones
-            const int depth = i % kScaleDepth;
-            wait(s, &s.sc_empty[depth], ((i / kScaleDepth) & 1) ^ 1);
-            named_bar_sync(3, 32 * kProducerWarps);  // every thread is done with the tables that are rewritten
-            const float top = largest(g, groups);
-            if (does_v) {
-                const int e = min(max(exponent(top), -15), 24);
-                store_groups(tv + (i & 1) * v_bytes + key_of * groups * 4, g, groups, exp2i(kTop - e));
-                reinterpret_cast<float*>(__cvta_shared_to_generic(s.base + s.l.key_v))[depth * kKeys + key_of] = e;
-                const __half w = __float2half_rn(exp2i(-e));
-                reinterpret_cast<__half*>(__cvta_shared_to_generic(s.base + s.l.key_w))[depth * kKeys + key_of] = w;
-            } else {
-                const int e = min(max(exponent(top), -100), 120);
-                store_groups(tk + key_of * groups * 4, g, groups, exp2i(kTop - e));
-                reinterpret_cast<float*>(__cvta_shared_to_generic(s.base + s.l.key_k))[depth * kKeys + key_of] = exp2i(e - kTop);
-            }
-            named_bar_sync(3, 32 * kProducerWarps);
-            if (pt == 0) mbar_arrive(&s.sc_full[depth]);
-            more = tw.next(a, next, next_first);
-            if (more) load_groups(next, does_v, key_of, groups, g);
-            emit(t, false, kr, tk);
-            if (more) load_codes(next, false, pt, kr);
-            if (have_prev) emit(prev, true, vr, tv + ((i - 1) & 1) * v_bytes);
-            load_codes(t, true, pt, vr);
-            prev = t;
-            have_prev = true;
-            if (!more) {
-                emit(prev, true, vr, tv + (i & 1) * v_bytes);
-                return;
-            }
-            t = next;
-            first = next_first;
+            --tile;  // the unit's last pass was V alone
+            cur = next;
         }
     }
 
     // ------------------------------------------------------------ products
-    __device__ static void issue(const Args& a, const Shared& s, Walker w, uint32_t tmem) {
+    __device__ static void issue(const Args& a, uint32_t tmem) {
         Ring ring{0, 0};
-        int tile = 0, units = 0;
-        Unit u;
-        const uint32_t q = s.base + s.l.q, p = s.base + s.l.p;
-        while (w.next(a, u)) {
-            const uint32_t n = u.rows <= 64 ? 64 : kRows;
-            const uint32_t desc_qk = tc5::shape(!kQuant, false, n), desc_pv = tc5::shape(!kQuant, true, n);
-            wait(s, s.q_full, units & 1);
+        int tile = 0;
+        const uint32_t q = smem_at(a.l.q), p = smem_at(a.l.p);
+#pragma unroll 1
+        for (int unit = 0;; ++unit) {
+            wait(&fixed().q_full, unit & 1);
             tc5::fence_after();
-            ++units;
+            const int tiles = *const_cast<volatile int*>(&fixed().unit_tiles);
+            const uint32_t n = *const_cast<volatile int*>(&fixed().unit_rows) <= 64 ? 64 : kRows;
+            if (tiles == 0) return;
+            const uint32_t desc_qk = tc5::shape(!kQuant, false, n), desc_pv = tc5::shape(!kQuant, true, n);
             const auto scores = [&](int i) {
                 const uint32_t d = tmem + ((tile + i) & 1) * a.nr;
+#pragma unroll 1
                 for (int b = 0; b < NB; ++b) {
-                    wait(s, &s.full[ring.slot], ring.phase);
+                    wait(&fixed().full[ring.slot], ring.phase);
                     tc5::fence_after();
-                    const uint32_t k = s.base + ring.slot * kBox, qb = q + b * a.nr * 128;
+                    const uint32_t k = smem_at(a.l.ring) + ring.slot * kBox, qb = q + b * a.nr * 128;
+                    const uint64_t dk = tc5::operand(k, 16, 1024), dq = tc5::operand(qb, 16, 1024);
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)
-                        tc5::mma(d, tc5::operand(k + ks * 32, 16, 1024), tc5::operand(qb + ks * 32, 16, 1024), desc_qk,
-                                 b + ks > 0);
-                    tc5::commit(&s.empty[ring.slot]);
+                    for (int ks = 0; ks < 4; ++ks) tc5::mma(d, dk + ks * 2, dq + ks * 2, desc_qk, b + ks > 0);  // 32 bytes on
+                    tc5::commit(&fixed().empty[ring.slot]);
                     ring.step(a.slots);
                 }
-                tc5::commit(&s.s_full[(tile + i) & 1]);
+                tc5::commit(&fixed().s_full[(tile + i) & 1]);
             };
-            scores(0);
-            for (int i = 0; i < u.n; ++i) {
-                if (i + 1 < u.n) scores(i + 1);
-                wait(s, s.p_full, (tile + i) & 1);
+#pragma unroll 1
+            for (int i = -1; i < tiles; ++i) {
+                if (i + 1 < tiles) scores(i + 1);
+                if (i < 0) continue;
+                wait(&fixed().p_full, (tile + i) & 1);
                 tc5::fence_after();
+#pragma unroll 1
                 for (int mb = 0; mb < MB; ++mb) {
                     const int slot = ring.slot;
                     int slot2 = slot;
-                    wait(s, &s.full[slot], ring.phase);
+                    wait(&fixed().full[slot], ring.phase);
                     ring.step(a.slots);
                     if (D > 64) {
                         slot2 = ring.slot;
-                        wait(s, &s.full[slot2], ring.phase);
+                        wait(&fixed().full[slot2], ring.phase);
                         ring.step(a.slots);
                     }
                     tc5::fence_after();
-                    const uint32_t v = s.base + slot * kBox;
+                    const uint64_t dv = tc5::operand(smem_at(a.l.ring) + slot * kBox, kBox, 1024);
+                    const uint64_t dp = tc5::operand(p, kBox, 1024);
 #pragma unroll
-                    for (int ks = 0; ks < kKeys / 16; ++ks)
-                        tc5::mma(tmem + (2 + mb) * a.nr, tc5::operand(v + ks * 2048, kBox, 1024),
-                                 tc5::operand(p + ks * 2048, kBox, 1024), desc_pv, i + ks > 0);
-                    tc5::commit(&s.empty[slot]);
-                    if (D > 64) tc5::commit(&s.empty[slot2]);
+                    for (int ks = 0; ks < kKeys / 16; ++ks)  // 16 keys of 128 bytes on
+                        tc5::mma(tmem + (2 + mb) * a.nr, dv + ks * 128, dp + ks * 128, desc_pv, i + ks > 0);
+                    tc5::commit(&fixed().empty[slot]);
+                    if (D > 64) tc5::commit(&fixed().empty[slot2]);
                 }
-                tc5::commit(s.pv_done);
+                tc5::commit(&fixed().pv_done);
             }
-            tile += u.n;
+            tile += tiles;
         }
     }
 
     // ------------------------------------------------------------ softmax
     // Q of a unit: rows of the block as K-major swizzled boxes; over quantised caches as fp16 scaled by a
     // power of two per row, in the order that the unpack leaves.
-    __device__ static __forceinline__ void load_q(const Args& a, const Shared& s, const Unit& u) {
+    __device__ static __forceinline__ void load_q(const Args& a, const Unit& u) {
         constexpr int kPieces = D / 8;
         const int tid = threadIdx.x;
         for (int idx = tid; idx < u.rows * kPieces; idx += 32 * kSoftmaxWarps) {
@@ -649,172 +685,175 @@ struct Kernel {
 #pragma unroll
                 for (int o = 1; o < kPieces && o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, o));
                 const int e = min(max(exponent(m), -100), 120);
-                const float sc = exp2i(kTop - e);
+                const float sc = exp2i(kTopQ - e);
                 uint32_t* p = &y.x;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) p[i] = pack2<false>(f[order<BITS>(2 * i)] * sc, f[order<BITS>(2 * i + 1)] * sc);
-                if (c == 0) s.qs[n] = a.scale * 1.4426950408889634f * exp2i(e - kTop);
+                if (c == 0) fixed().qs[n] = a.scale * 1.4426950408889634f * exp2i(e - kTopQ);
             }
-            sts128(s.base + s.l.q + (c >> 3) * a.nr * 128 + n * 128 + (((c & 7) ^ (n & 7)) << 4), y);
+            sts128(smem_at(a.l.q) + (c >> 3) * a.nr * 128 + n * 128 + (((c & 7) ^ (n & 7)) << 4), y);
         }
         if (tid < kRows) {
             const int n = tid, r = u.block * kRows + n;
             const bool live = n < u.rows;
-            s.thr[n] = live ? -INFINITY : INFINITY;  // a row that is not there never raises its maximum
-            s.mm[n] = -kLift;
-            s.m[n] = -INFINITY;
-            if (!kQuant) s.qs[n] = a.scale * 1.4426950408889634f;
-            int info = 0;
+            fixed().thr[n] = live ? -INFINITY : INFINITY;  // a row that is not there never raises its maximum
+            fixed().mm[n] = -kLift;
+            fixed().m[n] = -INFINITY;
+            // key b of the block (below 0: cached rows) is seen if b <= info, in a tree if bit b of info is set
+            int info = -1;
             if (live && !u.prefix) {
                 const int t = r / a.G;
                 info = a.parents ? static_cast<int>(tree_walk(a.parents + (size_t)u.seq * a.tokens, t).path) : t;
             }
-            s.rowinfo[n] = info;
+            fixed().info[n] = info;
         }
     }
 
-    __device__ static void softmax(const Args& a, const Shared& s, Walker w, uint32_t tmem, int cta) {
+    __device__ static void softmax(const Args& a, Walker w, uint32_t tmem, int cta) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3, half = warp >> 2;
         const int key = quarter * 32 + lane, tid = threadIdx.x & 127;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const int columns = a.nr / 2, c0 = half * columns;  // this warp's columns of S^T
         const int l_cols = a.nr / 8, l0 = warp * l_cols;    // columns whose sums it forms (inside its half)
-        const uint32_t ones = kQuant ? 0x3c003c00u : 0x3f803f80u;
+        constexpr uint32_t ones = 0x3f803f80u;
+        const float qscale = a.scale * 1.4426950408889634f;
         int tile = 0, units = 0;
         Unit u;
         while (w.next(a, u)) {
-            load_q(a, s, u);
+            load_q(a, u);
             fence_proxy_async_shared();
             tc5::fence_before();
             named_bar_sync(4, 32 * kSoftmaxWarps);
-            if (threadIdx.x == 0) mbar_arrive(s.q_full);
+            if (threadIdx.x == 0) {
+                fixed().unit_tiles = u.n;
+                fixed().unit_rows = u.rows;
+                mbar_arrive(&fixed().q_full);
+            }
             float lsum[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
             for (int i = 0; i < u.n; ++i, ++tile) {
                 const int depth = tile % kScaleDepth;
                 float ks = 1.f, ev = 0.f;
-                wait(s, &s.s_full[tile & 1], (tile >> 1) & 1);
+                wait(&fixed().s_full[tile & 1], (tile >> 1) & 1);
                 tc5::fence_after();
                 if (kQuant) {
-                    wait(s, &s.sc_full[depth], (tile / kScaleDepth) & 1);
-                    ks = reinterpret_cast<const float*>(__cvta_shared_to_generic(s.base + s.l.key_k))[depth * kKeys + key];
-                    ev = reinterpret_cast<const float*>(__cvta_shared_to_generic(s.base + s.l.key_v))[depth * kKeys + key];
+                    wait(&fixed().sc_full[depth], (tile / kScaleDepth) & 1);
+                    ks = fixed().key_k[depth][key];
+                    ev = fixed().key_v[depth][key];
                 }
-                const int at = (u.t0 + i) * kKeys, k_at = at + key;
-                const bool masked = at + kKeys > (u.prefix ? u.keys : u.len);
-                float y[2][32];
-                bool raise = false;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int n0 = c0 + 32 * c;
-                    if (32 * c < columns && n0 < u.rows) {
-                        tc5::ld32(tmem + lanes + (tile & 1) * a.nr + n0, y[c]);
+                const int at = (u.t0 + i) * kKeys;
+                const int b = at + key - u.len;  // block row of the key; a prefix ends where its block would begin
+                const bool masked = at + kKeys > u.len;
+                bool waited = i == 0;  // for the last tile's p V: P and the accumulators are free
+#pragma unroll 1
+                for (int n0 = c0; n0 < min(c0 + columns, u.rows); n0 += 32) {  // 32 columns at a time in registers
+                    float y[32];
+                    bool raise = false;
+                    tc5::ld32(tmem + lanes + (tile & 1) * a.nr + n0, y);
+                    if (kQuant) {
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
-                            const float4 th = *reinterpret_cast<const float4*>(&s.thr[n0 + j]);
-                            const float4 qs = *reinterpret_cast<const float4*>(&s.qs[n0 + j]);
-                            const float t4[4] = {th.x, th.y, th.z, th.w}, q4[4] = {qs.x, qs.y, qs.z, qs.w};
+                            const float4 qs = *reinterpret_cast<const float4*>(&fixed().qs[n0 + j]);
+                            y[j] = fmaf(y[j] * ks, qs.x, ev);
+                            y[j + 1] = fmaf(y[j + 1] * ks, qs.y, ev);
+                            y[j + 2] = fmaf(y[j + 2] * ks, qs.z, ev);
+                            y[j + 3] = fmaf(y[j + 3] * ks, qs.w, ev);
+                        }
+                    } else {
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) {
-                                float v = kQuant ? fmaf(y[c][j + x] * ks, q4[x], ev) : y[c][j + x] * q4[x];
-                                if (masked) {
-                                    const int b = k_at - u.len;  // block row of the key
-                                    const int info = s.rowinfo[n0 + j + x];
-                                    const bool seen = k_at < u.len || (!u.prefix && k_at < u.keys &&
-                                                                       (a.parents ? (info >> b) & 1 : b <= info));
-                                    v = seen ? v : -INFINITY;
-                                }
-                                raise = raise || v > t4[x];
-                                y[c][j + x] = v;
-                            }
+                        for (int j = 0; j < 32; ++j) y[j] *= qscale;
+                    }
+                    if (masked) {  // by the row's token, or its path's bits (load_q)
+                        if (a.parents && !u.prefix) {
+                            const int bit = b < 0 ? -1 : b < 32 ? 1 << b : 0;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) y[j] = fixed().info[n0 + j] & bit ? y[j] : -INFINITY;
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) y[j] = b <= fixed().info[n0 + j] ? y[j] : -INFINITY;
                         }
                     }
-                }
-                bool waited = i == 0;
-                if (bar_any(1 + half, 128, raise)) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int n0 = c0 + 32 * c;
-                        if (32 * c < columns && n0 < u.rows) {
-                            float mine = -INFINITY;
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const float m = warp_max(y[c][j]);
-                                if (lane == j) mine = m;
-                            }
-                            s.part[quarter * kRows + n0 + lane] = mine;
-                        }
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 th = *reinterpret_cast<const float4*>(&fixed().thr[n0 + j]);
+                        raise = raise || y[j] > th.x || y[j + 1] > th.y || y[j + 2] > th.z || y[j + 3] > th.w;
                     }
-                    named_bar_sync(1 + half, 128);
-                    if (tid < columns && c0 + tid < u.rows) {
-                        const int n = c0 + tid;
-                        const float old = s.m[n];
-                        const float m = fmaxf(fmaxf(fmaxf(s.part[n], s.part[kRows + n]),
-                                                    fmaxf(s.part[2 * kRows + n], s.part[3 * kRows + n])), old);
-                        s.corr[n] = m == old ? 1.f : ex2(old - m);
-                        s.m[n] = m;
-                        s.thr[n] = m + kLazy;
-                        s.mm[n] = (m == -INFINITY ? 0.f : m) - kLift;
-                    }
-                    named_bar_sync(1 + half, 128);
-                    if (!waited) {  // the accumulators so far go to the new maxima
-                        wait(s, s.pv_done, (tile - 1) & 1);
+                    raise = bar_any(1 + half, 128, raise);
+                    if (!waited) {
+                        wait(&fixed().pv_done, (tile - 1) & 1);
                         tc5::fence_after();
                         waited = true;
-                        if (D > 64 || quarter < 2) {
+                    }
+                    if (raise) {
+                        float mine = -INFINITY;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float m = warp_max(y[j]);
+                            if (lane == j) mine = m;
+                        }
+                        fixed().part[quarter][n0 + lane] = mine;
+                        named_bar_sync(1 + half, 128);
+                        if (tid < 32 && n0 + tid < u.rows) {
+                            const int n = n0 + tid;
+                            const float old = fixed().m[n];
+                            const float m = fmaxf(fmaxf(fmaxf(fixed().part[0][n], fixed().part[1][n]),
+                                                        fmaxf(fixed().part[2][n], fixed().part[3][n])), old);
+                            fixed().corr[n] = m == old ? 1.f : ex2(old - m);
+                            fixed().m[n] = m;
+                            fixed().thr[n] = m + kLazy;
+                            fixed().mm[n] = (m == -INFINITY ? 0.f : m) - kLift;
+                        }
+                        named_bar_sync(1 + half, 128);
+                        if (i > 0 && (D > 64 || quarter < 2)) {  // the accumulators so far go to the new maxima
                             for (int mb = 0; mb < MB; ++mb)
-                                for (int n0 = c0; n0 < min(c0 + columns, u.rows); n0 += 16) {
+                                for (int n1 = n0; n1 < min(n0 + 32, u.rows); n1 += 16) {
                                     uint32_t r[16];
-                                    const uint32_t addr = tmem + lanes + (2 + mb) * a.nr + n0;
+                                    const uint32_t addr = tmem + lanes + (2 + mb) * a.nr + n1;
                                     tc5::ld16(addr, r);
 #pragma unroll
                                     for (int j = 0; j < 16; ++j)
-                                        r[j] = __float_as_uint(__uint_as_float(r[j]) * (n0 + j < u.rows ? s.corr[n0 + j] : 1.f));
+                                        r[j] = __float_as_uint(__uint_as_float(r[j]) *
+                                                               (n1 + j < u.rows ? fixed().corr[n1 + j] : 1.f));
                                     tc5::st16(addr, r);
                                 }
                             tc5::wait_st();
                         }
-                    }
 #pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        if (8 * x < l_cols) {
+                        for (int x = 0; x < 2; ++x) {  // and the sums, each warp its own columns
                             const int n = l0 + 8 * x + 2 * (lane & 3);
-                            if (n < u.rows) lsum[x][0] *= s.corr[n];
-                            if (n + 1 < u.rows) lsum[x][1] *= s.corr[n + 1];
-                        }
-                }
-                if (!waited) {
-                    wait(s, s.pv_done, (tile - 1) & 1);  // P is free again
-                    tc5::fence_after();
-                }
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int n0 = c0 + 32 * c;
-                    if (32 * c < columns && n0 < u.rows) {
-                        const uint32_t row = s.base + s.l.p + (n0 >> 6) * kBox + key * 128;
-#pragma unroll
-                        for (int j = 0; j < 32; j += 8) {
-                            const float4 ma = *reinterpret_cast<const float4*>(&s.mm[n0 + j]);
-                            const float4 mb = *reinterpret_cast<const float4*>(&s.mm[n0 + j + 4]);
-                            uint4 v;
-                            v.x = pack2<!kQuant>(ex2(y[c][j] - ma.x), ex2(y[c][j + 1] - ma.y));
-                            v.y = pack2<!kQuant>(ex2(y[c][j + 2] - ma.z), ex2(y[c][j + 3] - ma.w));
-                            v.z = pack2<!kQuant>(ex2(y[c][j + 4] - mb.x), ex2(y[c][j + 5] - mb.y));
-                            v.w = pack2<!kQuant>(ex2(y[c][j + 6] - mb.z), ex2(y[c][j + 7] - mb.w));
-                            sts128(row + (((((n0 & 63) + j) >> 3) ^ (key & 7)) << 4), v);
+                            if (8 * x < l_cols && n >= n0 && n < n0 + 32) {
+                                if (n < u.rows) lsum[x][0] *= fixed().corr[n];
+                                if (n + 1 < u.rows) lsum[x][1] *= fixed().corr[n + 1];
+                            }
                         }
                     }
+                    const uint32_t row = smem_at(a.l.p) + (n0 >> 6) * kBox + key * 128;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        const float4 ma = *reinterpret_cast<const float4*>(&fixed().mm[n0 + j]);
+                        const float4 mb = *reinterpret_cast<const float4*>(&fixed().mm[n0 + j + 4]);
+                        uint4 v;
+                        v.x = pack2<!kQuant>(ex2(y[j] - ma.x), ex2(y[j + 1] - ma.y));
+                        v.y = pack2<!kQuant>(ex2(y[j + 2] - ma.z), ex2(y[j + 3] - ma.w));
+                        v.z = pack2<!kQuant>(ex2(y[j + 4] - mb.x), ex2(y[j + 5] - mb.y));
+                        v.w = pack2<!kQuant>(ex2(y[j + 6] - mb.z), ex2(y[j + 7] - mb.w));
+                        sts128(row + (((((n0 & 63) + j) >> 3) ^ (key & 7)) << 4), v);
+                    }
+                }
+                if (!waited) {  // no columns of its own
+                    wait(&fixed().pv_done, (tile - 1) & 1);
+                    tc5::fence_after();
                 }
                 fence_proxy_async_shared();
                 tc5::fence_before();
                 named_bar_sync(1 + half, 128);
-                if (tid == 0) mbar_arrive(s.p_full);
+                if (tid == 0) mbar_arrive(&fixed().p_full);
                 // sums of the columns over the tile's keys: one 16-row product with a row of ones (or of
                 // the keys' weights), on the rounded P that the numerator uses
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const int n = l0 + 8 * x;
                     if (8 * x < l_cols && n < u.rows) {
-                        const uint32_t box = s.base + s.l.p + (n >> 6) * kBox;
+                        const uint32_t box = smem_at(a.l.p) + (n >> 6) * kBox;
 #pragma unroll
                         for (int kk = 0; kk < kKeys; kk += 32) {
                             const int r = kk + lane;
@@ -824,7 +863,7 @@ struct Kernel {
                                          : "r"(box + r * 128 + (((((n & 63) >> 3)) ^ (r & 7)) << 4))
                                          : "memory");
                             if constexpr (kQuant) {
-                                const uint32_t kw = s.base + s.l.key_w + (depth * kKeys + kk + 2 * (lane & 3)) * 2;
+                                const uint32_t kw = smem_u32(&fixed().key_w[depth][kk + 2 * (lane & 3)]);
                                 const uint32_t a0 = lds32(kw), a2 = lds32(kw + 16), a4 = lds32(kw + 32), a6 = lds32(kw + 48);
                                 mma_f16_16816(lsum[x], a0, a0, a2, a2, b0, b1);
                                 mma_f16_16816(lsum[x], a4, a4, a6, a6, b2, b3);
@@ -837,11 +876,11 @@ struct Kernel {
                 }
                 if (kQuant) {
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&s.sc_empty[depth]);
+                    if (lane == 0) mbar_arrive(&fixed().sc_empty[depth]);
                 }
             }
             // the unit's partial
-            wait(s, s.pv_done, (tile - 1) & 1);
+            wait(&fixed().pv_done, (tile - 1) & 1);
             tc5::fence_after();
             const long long at = partial_row(a, u.prefix, u.segment, cta);
             if (D > 64 || quarter < 2) {
@@ -862,15 +901,15 @@ struct Kernel {
                 for (int x = 0; x < 2; ++x)
                     if (8 * x < l_cols) {
                         const int n = l0 + 8 * x + 2 * lane;
-                        if (n < u.rows) a.ml[at + n] = make_float2(s.m[n], lsum[x][0]);
-                        if (n + 1 < u.rows) a.ml[at + n + 1] = make_float2(s.m[n + 1], lsum[x][1]);
+                        if (n < u.rows) a.ml[at + n] = make_float2(fixed().m[n], lsum[x][0]);
+                        if (n + 1 < u.rows) a.ml[at + n + 1] = make_float2(fixed().m[n + 1], lsum[x][1]);
                     }
             }
             if (threadIdx.x == 0) {
                 const long long seg = (u.prefix ? 0 : segments_p(a)) + u.segment;
                 if (u.t0 == 0) a.first[seg] = cta;
                 if (u.t0 + u.n == u.tiles) a.last[seg] = cta;
-                int* flag = &s.poison[units & (kPoison - 1)];
+                int* flag = &fixed().poison[units & (kPoison - 1)];
                 a.poison[partial_index(a, u.prefix, u.segment, cta)] = *reinterpret_cast<volatile int*>(flag);
                 *flag = 0;
             }
@@ -878,10 +917,14 @@ struct Kernel {
             tc5::fence_before();
             named_bar_sync(4, 32 * kSoftmaxWarps);  // Q, the row arrays and the accumulators are free
         }
+        if (threadIdx.x == 0) {
+            fixed().unit_tiles = 0;
+            mbar_arrive(&fixed().q_full);
+        }
     }
 
     // The CTA's run of tiles: a scan over the entries' tile counts.
-    __device__ static void plan(const Args& a, int* misc) {
+    __device__ static void plan(const Args& a) {
         const int entries = a.cache.sequences * a.blocks_o, tid = threadIdx.x;
         const int per = (entries + kThreads - 1) / kThreads;
         const int e0 = min(entries, tid * per), e1 = min(entries, e0 + per);
@@ -891,7 +934,7 @@ struct Kernel {
             if (e % a.blocks_o == 0 && blockIdx.x == 0) kv::block_start(a.lengths, e / a.blocks_o, a.tokens, a.cache.max_len);
             sum += entry_tiles(a, e) * a.cache.hkv;
         }
-        int* s_warp = misc + 8;
+        int* s_warp = fixed().warp_sum;
         const int warp = tid >> 5, lane = tid & 31;
         int scan = sum;
 #pragma unroll
@@ -913,9 +956,9 @@ struct Kernel {
         const int w1 = cta < ctas ? static_cast<int>((long long)total * (cta + 1) / ctas) : 0;
         const int w = max(w0, prefix_end);  // first own tile of the run
         if (tid == 0) {
-            misc[2] = w0;
-            misc[3] = w1;
-            misc[4] = misc[5] = 0;
+            fixed().w0 = w0;
+            fixed().w1 = w1;
+            fixed().entry = fixed().off = 0;
         }
         __syncthreads();
         if (w < w1 && before <= w && w < before + sum) {
@@ -924,70 +967,58 @@ struct Kernel {
                 off += n;
                 n = entry_tiles(a, ++e) * a.cache.hkv;
             }
-            misc[4] = e;
-            misc[5] = off;
+            fixed().entry = e;
+            fixed().off = off;
         }
     }
 
     __device__ static void run(const Args& a) {
-        extern __shared__ __align__(1024) uint8_t smem[];
-        Shared s;
-        s.base = (smem_u32(smem) + 1023u) & ~1023u;
-        s.l = layout(D, a.nr, a.slots, kQuant ? D / a.cache.group : 0);
-        uint8_t* g = smem + (s.base - smem_u32(smem));
-        s.full = reinterpret_cast<uint64_t*>(g + s.l.bars);
-        s.empty = s.full + kMaxSlots;
-        s.s_full = s.empty + kMaxSlots;
-        s.p_full = s.s_full + 2;
-        s.pv_done = s.p_full + 1;
-        s.q_full = s.pv_done + 1;
-        s.sc_full = s.q_full + 1;
-        s.sc_empty = s.sc_full + kScaleDepth;
-        s.poison = reinterpret_cast<int*>(g + s.l.misc);
-        s.misc = s.poison + kPoison;
-        s.abort = s.misc;
-        s.thr = reinterpret_cast<float*>(g + s.l.row);
-        s.mm = s.thr + kRows;
-        s.qs = s.mm + kRows;
-        s.corr = s.qs + kRows;
-        s.m = s.corr + kRows;
-        s.rowinfo = reinterpret_cast<int*>(s.m + kRows);
-        s.part = reinterpret_cast<float*>(g + s.l.part);
+        if (smem_at(0) & 1023u) {  // the swizzled boxes need it; every thread leaves here
+            if (threadIdx.x == 0) atomicOr(&g_device_error, DFLASH_DEVERR_ATTN_PIPELINE);
+            return;
+        }
         const int warp = threadIdx.x >> 5;
         if (threadIdx.x == 0) {
             for (int i = 0; i < kMaxSlots; ++i) {
-                mbar_init(&s.full[i], kProducerWarps);
-                mbar_init(&s.empty[i], 1);
+                mbar_init(&fixed().full[i], kProducerWarps);
+                mbar_init(&fixed().empty[i], 1);
             }
-            mbar_init(&s.s_full[0], 1);
-            mbar_init(&s.s_full[1], 1);
-            mbar_init(s.p_full, 2);
-            mbar_init(s.pv_done, 1);
-            mbar_init(s.q_full, 1);
+            mbar_init(&fixed().s_full[0], 1);
+            mbar_init(&fixed().s_full[1], 1);
+            mbar_init(&fixed().p_full, 2);
+            mbar_init(&fixed().pv_done, 1);
+            mbar_init(&fixed().q_full, 1);
             for (int i = 0; i < kScaleDepth; ++i) {
-                mbar_init(&s.sc_full[i], 1);
-                mbar_init(&s.sc_empty[i], kSoftmaxWarps);
+                mbar_init(&fixed().sc_full[i], 1);
+                mbar_init(&fixed().sc_empty[i], kSoftmaxWarps);
             }
-            s.misc[0] = 0;
+            fixed().abort = 0;
             fence_barrier_init();
         }
-        if (threadIdx.x < kPoison) s.poison[threadIdx.x] = 0;
-        if (warp == kSoftmaxWarps + kProducerWarps) tc5::alloc(smem_u32(&s.misc[1]), kTmemColumns);
+        if (threadIdx.x < kPoison) fixed().poison[threadIdx.x] = 0;
+        if (warp == kSoftmaxWarps + kProducerWarps) tc5::alloc(smem_u32(&fixed().tmem), kTmemColumns);
         pdl_wait();
         pdl_launch_dependents();
-        plan(a, s.misc);
+        plan(a);
         tc5::fence_before();
         __syncthreads();
         tc5::fence_after();
-        const uint32_t tmem = *reinterpret_cast<volatile int*>(&s.misc[1]);
-        const Walker w{s.misc[2], s.misc[3], s.misc[4], s.misc[5]};
+        const uint32_t tmem = *reinterpret_cast<volatile int*>(&fixed().tmem);
+        const Walker w{fixed().w0, fixed().w1, fixed().entry, fixed().off};
         if (warp < kSoftmaxWarps) {
-            softmax(a, s, w, tmem, blockIdx.x);
+            if constexpr (!kQuant) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(120));
+            softmax(a, w, tmem, blockIdx.x);
         } else if (warp < kSoftmaxWarps + kProducerWarps) {
-            if constexpr (kQuant) produce_quant(a, s, w);
-            else produce_bf16(a, s, w);
+            if constexpr (kQuant) {
+                asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(120));
+                produce_quant(a, w);
+            } else {
+                asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(72));
+                produce_bf16(a, w);
+            }
         } else {
-            if ((threadIdx.x & 31) == 0) issue(a, s, w, tmem);
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+            if (threadIdx.x == 32 * (kSoftmaxWarps + kProducerWarps)) issue(a, tmem);
             __syncwarp();
         }
         tc5::fence_before();
@@ -1080,7 +1111,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     poison = __any_sync(0xffffffffu, poison != 0);
-    const float inv = (BITS == 16 ? 1.f : exp2i(-kTop)) / l;
+    const float inv = (BITS == 16 ? 1.f : exp2i(-Kernel<BITS, D>::kTop)) / l;
 #pragma unroll
     for (int i = 0; i < CH; ++i) acc[i] *= inv;
     if (poison) {  // block rows whose values were taken out: they reach the rows that see them
@@ -1146,6 +1177,7 @@ static size_t fit(Args& a, const dflash_kv_cache& c, int prefix_len, int tokens,
     const int groups = c.bits == 16 ? 0 : c.head_dim / c.group;
     a.slots = kMaxSlots;
     while (layout(c.head_dim, a.nr, a.slots, groups).total > kSmemLimit) a.slots -= 2;
+    a.l = layout(c.head_dim, a.nr, a.slots, groups);
     size_t at = 0;
     const auto take = [&](size_t bytes) {
         uint8_t* p = base + at;
@@ -1164,11 +1196,9 @@ static size_t fit(Args& a, const dflash_kv_cache& c, int prefix_len, int tokens,
 
 template <int BITS, int D>
 static cudaError_t launch(const Args& a, int ctas, cudaStream_t s) {
-    const int groups = BITS == 16 ? 0 : D / a.cache.group;
-    const size_t smem = layout(D, a.nr, a.slots, groups).total + 1024;
-    cudaError_t e = cudaFuncSetAttribute(attn_batch_kernel<BITS, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+    cudaError_t e = cudaFuncSetAttribute(attn_batch_kernel<BITS, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
     if (e != cudaSuccess) return e;
-    e = launch_chained(attn_batch_kernel<BITS, D>, dim3(ctas), dim3(kThreads), smem, s, 1, a);
+    e = launch_chained(attn_batch_kernel<BITS, D>, dim3(ctas), dim3(kThreads), a.l.total, s, 1, a);
     if (e != cudaSuccess) return e;
     const long long items = (long long)a.cache.sequences * a.tokens * a.hq;
     return launch_chained(attn_join_kernel<BITS, D>, dim3(static_cast<unsigned>((items + 7) / 8)), dim3(256), 0, s, 1, a);
