@@ -225,9 +225,11 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool fill) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(fill ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// Arrives on the mbarrier (one of its expected arrivals) once this thread's copies so far are complete.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 // bar.red.or over `threads` threads of barrier `id`.
 __device__ __forceinline__ bool bar_any(int id, int threads, bool v) {
     uint32_t r;
@@ -333,8 +335,9 @@ struct Kernel {
         }
     };
 
+    // The writes become visible to the tensor cores through the proxy fence of the thread that waits for
+    // them (issue): a fence here would wait for this warp's loads in flight as well.
     __device__ static __forceinline__ void signal_full(int slot) {
-        fence_proxy_async_shared();
         __syncwarp();
         if ((threadIdx.x & 31) == 0) mbar_arrive(&fixed().full[slot]);
     }
@@ -369,33 +372,12 @@ struct Kernel {
         }
     }
 
-    // bf16 caches: cp.async straight into the swizzled boxes, up to kLag boxes in flight.
-    static constexpr int kLag = 5;
-
+    // bf16 caches: cp.async straight into the swizzled boxes; the copies themselves arrive on the box's
+    // barrier, so as many boxes are in flight as the ring has free slots.
     __device__ static void produce_bf16(const Args& a, Walker w) {
         const int pt = threadIdx.x - 32 * kSoftmaxWarps, key0 = pt >> 3, c = pt & 7;
         const uint32_t ring_at = smem_at(a.l.ring), dst0 = ring_at + key0 * 128 + ((c ^ (key0 & 7)) << 4);
         Ring ring{0, 0};
-        int done_slot = 0, pending = 0;
-        int from[kLag] = {}, flag[kLag] = {};  // what to look at in the boxes in flight, oldest first
-        const auto retire_oldest = [&]() {
-            switch (pending) {
-                case 1: cp_async_wait<0>(); break;
-                case 2: cp_async_wait<1>(); break;
-                case 3: cp_async_wait<2>(); break;
-                case 4: cp_async_wait<3>(); break;
-                default: cp_async_wait<4>(); break;
-            }
-            if (__builtin_expect(from[0] < kKeys, 0)) take_out(ring_at + done_slot * kBox, from[0], pt, &fixed().poison[flag[0]]);
-            signal_full(done_slot);
-            if (++done_slot == a.slots) done_slot = 0;
-#pragma unroll
-            for (int i = 0; i + 1 < kLag; ++i) {
-                from[i] = from[i + 1];
-                flag[i] = flag[i + 1];
-            }
-            --pending;
-        };
         Unit u;
         for (int unit = 0; w.next(a, u); ++unit) {
             const Source src(a, u);
@@ -408,32 +390,24 @@ struct Kernel {
                 const uint8_t* p = (is_v ? src.v : src.k) + ((int64_t)(key_at + key0) * D + c * 8) * 2;
 #pragma unroll 1
                 for (int b = 0; b < NB; ++b, p += 128) {
-                    if (pending == kLag) retire_oldest();
-                    while (!mbar_try_wait(&fixed().empty[ring.slot], ring.phase ^ 1)) {
-                        if (pending == 0) {
-                            wait(&fixed().empty[ring.slot], ring.phase ^ 1);
-                            break;
-                        }
-                        retire_oldest();
-                    }
+                    wait(&fixed().empty[ring.slot], ring.phase ^ 1);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const bool live = key0 + 32 * x < valid;
                         cp_async16(dst0 + ring.slot * kBox + x * 4096, live ? p + x * (32 * D * 2) : src.k, live);
                     }
-                    cp_async_commit();
-#pragma unroll
-                    for (int x = 0; x < kLag; ++x)
-                        if (x == pending) {
-                            from[x] = is_v && look < valid ? look : kKeys;
-                            flag[x] = unit & (kPoison - 1);
-                        }
-                    ++pending;
+                    if (__builtin_expect(is_v && look < valid, 0)) {
+                        cp_async_wait_all();
+                        take_out(ring_at + ring.slot * kBox, look, pt, &fixed().poison[unit & (kPoison - 1)]);
+                        mbar_arrive(&fixed().full[ring.slot]);
+                    } else {
+                        cp_async_arrive(&fixed().full[ring.slot]);
+                    }
                     ring.step(a.slots);
                 }
             }
         }
-        while (pending > 0) retire_oldest();
+        cp_async_wait_all();  // nothing is in flight when the block's shared memory goes
     }
 
     // Quantised caches: codes to registers a tile ahead, unpacked to fp16 and stored swizzled.
@@ -601,7 +575,11 @@ struct Kernel {
     }
 
     // ------------------------------------------------------------ products
-    __device__ static void issue(const Args& a, uint32_t tmem) {
+    // Run by a whole warp, so that addresses and descriptors stay in uniform registers; one elected lane
+    // issues.  What comes from shared memory is broadcast for the same reason.
+    __device__ static void issue(const Args& a, uint32_t tmem_lane) {
+        const bool one = tc5::elect();
+        const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_lane, 0);
         Ring ring{0, 0};
         int tile = 0;
         const uint32_t q = smem_at(a.l.q), p = smem_at(a.l.p);
@@ -609,8 +587,9 @@ struct Kernel {
         for (int unit = 0;; ++unit) {
             wait(&fixed().q_full, unit & 1);
             tc5::fence_after();
-            const int tiles = *const_cast<volatile int*>(&fixed().unit_tiles);
-            const uint32_t n = *const_cast<volatile int*>(&fixed().unit_rows) <= 64 ? 64 : kRows;
+            const int tiles = __shfl_sync(0xffffffffu, *const_cast<volatile int*>(&fixed().unit_tiles), 0);
+            const int rows = __shfl_sync(0xffffffffu, *const_cast<volatile int*>(&fixed().unit_rows), 0);
+            const uint32_t n = rows <= 64 ? 64 : kRows;
             if (tiles == 0) return;
             const uint32_t desc_qk = tc5::shape(!kQuant, false, n), desc_pv = tc5::shape(!kQuant, true, n);
             const auto scores = [&](int i) {
@@ -618,15 +597,17 @@ struct Kernel {
 #pragma unroll 1
                 for (int b = 0; b < NB; ++b) {
                     wait(&fixed().full[ring.slot], ring.phase);
-                    tc5::fence_after();
+                    fence_proxy_async_shared();
                     const uint32_t k = smem_at(a.l.ring) + ring.slot * kBox, qb = q + b * a.nr * 128;
                     const uint64_t dk = tc5::operand(k, 16, 1024), dq = tc5::operand(qb, 16, 1024);
+                    if (one) {
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) tc5::mma(d, dk + ks * 2, dq + ks * 2, desc_qk, b + ks > 0);  // 32 bytes on
-                    tc5::commit(&fixed().empty[ring.slot]);
+                        for (int ks = 0; ks < 4; ++ks) tc5::mma(d, dk + ks * 2, dq + ks * 2, desc_qk, b + ks > 0);  // 32 bytes on
+                        tc5::commit(&fixed().empty[ring.slot]);
+                    }
                     ring.step(a.slots);
                 }
-                tc5::commit(&fixed().s_full[(tile + i) & 1]);
+                if (one) tc5::commit(&fixed().s_full[(tile + i) & 1]);
             };
 #pragma unroll 1
             for (int i = -1; i < tiles; ++i) {
@@ -645,16 +626,19 @@ struct Kernel {
                         wait(&fixed().full[slot2], ring.phase);
                         ring.step(a.slots);
                     }
-                    tc5::fence_after();
+                    fence_proxy_async_shared();
                     const uint64_t dv = tc5::operand(smem_at(a.l.ring) + slot * kBox, kBox, 1024);
                     const uint64_t dp = tc5::operand(p, kBox, 1024);
+                    const uint32_t d = tmem + (2 + mb) * a.nr;
+                    if (one) {
 #pragma unroll
-                    for (int ks = 0; ks < kKeys / 16; ++ks)  // 16 keys of 128 bytes on
-                        tc5::mma(tmem + (2 + mb) * a.nr, dv + ks * 128, dp + ks * 128, desc_pv, i + ks > 0);
-                    tc5::commit(&fixed().empty[slot]);
-                    if (D > 64) tc5::commit(&fixed().empty[slot2]);
+                        for (int ks = 0; ks < kKeys / 16; ++ks)  // 16 keys of 128 bytes on
+                            tc5::mma(d, dv + ks * 128, dp + ks * 128, desc_pv, i + ks > 0);
+                        tc5::commit(&fixed().empty[slot]);
+                        if (D > 64) tc5::commit(&fixed().empty[slot2]);
+                    }
                 }
-                tc5::commit(&fixed().pv_done);
+                if (one) tc5::commit(&fixed().pv_done);
             }
             tile += tiles;
         }
@@ -747,7 +731,6 @@ struct Kernel {
 #pragma unroll 1
                 for (int n0 = c0; n0 < min(c0 + columns, u.rows); n0 += 32) {  // 32 columns at a time in registers
                     float y[32];
-                    bool raise = false;
                     tc5::ld32(tmem + lanes + (tile & 1) * a.nr + n0, y);
                     if (kQuant) {
 #pragma unroll
@@ -772,12 +755,16 @@ struct Kernel {
                             for (int j = 0; j < 32; ++j) y[j] = b <= fixed().info[n0 + j] ? y[j] : -INFINITY;
                         }
                     }
+                    bool over[4] = {false, false, false, false};
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
                         const float4 th = *reinterpret_cast<const float4*>(&fixed().thr[n0 + j]);
-                        raise = raise || y[j] > th.x || y[j + 1] > th.y || y[j + 2] > th.z || y[j + 3] > th.w;
+                        over[0] |= y[j] > th.x;
+                        over[1] |= y[j + 1] > th.y;
+                        over[2] |= y[j + 2] > th.z;
+                        over[3] |= y[j + 3] > th.w;
                     }
-                    raise = bar_any(1 + half, 128, raise);
+                    const bool raise = bar_any(1 + half, 128, (over[0] | over[1]) | (over[2] | over[3]));
                     if (!waited) {
                         wait(&fixed().pv_done, (tile - 1) & 1);
                         tc5::fence_after();
@@ -977,10 +964,10 @@ struct Kernel {
             if (threadIdx.x == 0) atomicOr(&g_device_error, DFLASH_DEVERR_ATTN_PIPELINE);
             return;
         }
-        const int warp = threadIdx.x >> 5;
+        const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
         if (threadIdx.x == 0) {
             for (int i = 0; i < kMaxSlots; ++i) {
-                mbar_init(&fixed().full[i], kProducerWarps);
+                mbar_init(&fixed().full[i], kQuant ? kProducerWarps : 32 * kProducerWarps);
                 mbar_init(&fixed().empty[i], 1);
             }
             mbar_init(&fixed().s_full[0], 1);
@@ -1018,7 +1005,7 @@ struct Kernel {
             }
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-            if (threadIdx.x == 32 * (kSoftmaxWarps + kProducerWarps)) issue(a, tmem);
+            if (warp == kSoftmaxWarps + kProducerWarps) issue(a, tmem);
             __syncwarp();
         }
         tc5::fence_before();
