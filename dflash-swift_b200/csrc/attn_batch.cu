@@ -21,7 +21,7 @@
 //
 // Roles: warps 0-7 softmax (two per TMEM lane quarter, half of the columns each), 8-15 producers
 // (cache rows to swizzled shared memory boxes of 128 keys x 64 elements, in a ring), warp 16 issues
-// the products (17-19 have no work).  The running maximum is only raised when a score passes it by kLazy (in powers
+// the products, warp 17 the bulk copies of codes to staging slots (18 and 19 have no work).  The running maximum is only raised when a score passes it by kLazy (in powers
 // of two), so the accumulators are rarely rescaled.
 #include "common.cuh"
 #include "dflash_batch.h"
@@ -38,12 +38,11 @@ constexpr int kBox = kKeys * 128;          // bytes of a ring slot: 128 keys x 6
 constexpr int kSoftmaxWarps = 8, kProducerWarps = 8;
 constexpr int kThreads = 32 * (kSoftmaxWarps + kProducerWarps + 4);  // whole warpgroups: registers move between them
 // Registers a thread.  The block starts with kThreads x 96 = 61440 and every warpgroup takes or gives; what is
-// taken is never more than what is given, so nobody waits for good:
-//   quantised: 256 x 96 + 256 x 120 + 128 x 40 = 60416 (the producers hold two tiles of codes),
-//   bf16:     256 x 120 + 256 x 72 + 128 x 40 = 54272.
-constexpr int kIssueRegs = 40;
+// taken is never more than what is given, so nobody waits for good: 256 x 112 + 256 x 80 + 128 x 72 = 58368.
+constexpr int kSoftmaxRegs = 112, kProducerRegs = 80, kIssueRegs = 72;
 constexpr int kMaxCtas = 160;              // partials are sized for this many CTAs
 constexpr int kMaxSlots = 10;
+constexpr int kMaxStages = 8;              // staging slots for codes, 64 d bytes each
 constexpr int kScaleDepth = 4;             // tiles whose key factors may be alive at once
 constexpr int kPoison = 16;                // units whose poison flags may be alive at once
 constexpr float kLazy = 4.f;               // a maximum moves when a score passes it by 2^4 ...
@@ -56,7 +55,7 @@ constexpr int kSmemLimit = 232448;
 // tables, and from the next 1024-byte border on the ring, Q and P.
 struct Fixed {
     uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full, pv_done, q_full, sc_full[kScaleDepth],
-        sc_empty[kScaleDepth];
+        sc_empty[kScaleDepth], staged[kMaxStages], unstaged[kMaxStages];
     alignas(16) float thr[kRows];       // read four at a time, like mm and qs
     float mm[kRows], qs[kRows], corr[kRows], m[kRows];
     int info[kRows];                    // chain: the row's token; tree: its path mask
@@ -73,14 +72,15 @@ static_assert(offsetof(Fixed, thr) % 16 == 0 && offsetof(Fixed, mm) % 16 == 0 &&
 constexpr uint32_t kTables = (sizeof(Fixed) + 15) / 16 * 16;
 
 struct Layout {
-    uint32_t ring, q, p, total;
+    uint32_t ring, q, p, stage, total;
 };
-__host__ inline Layout layout(int d, int nr, int slots, int groups) {
+__host__ inline Layout layout(int d, int nr, int slots, int stages, int groups) {
     Layout l;
     l.ring = (kTables + 3 * kKeys * groups * 4 + 1023) / 1024 * 1024;
     l.q = l.ring + slots * kBox;
     l.p = l.q + nr * d * 2;
-    l.total = l.p + kKeys * nr * 2;
+    l.stage = l.p + kKeys * nr * 2;
+    l.total = l.stage + stages * 64 * d;
     return l;
 }
 
@@ -98,7 +98,7 @@ struct Args {
     int G, blocks_p, blocks_o;   // row blocks of the prefix and of one sequence
     int rows_o;                  // rows of a block of one sequence, at most
     int nr;                      // columns of the products' buffers: 64 or kRows
-    int slots;                   // ring slots
+    int slots, stages;           // ring slots, staging slots (quantised caches)
     Layout l;
     // workspace: partials of the prefix, then of the sequences
     int32_t* first;              // [segments] first and last CTA of each (row block, kv head)
@@ -230,6 +230,12 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// Copies `bytes` (a multiple of 16, 16-byte aligned on both sides) to shared memory; they count on the mbarrier.
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
 // bar.red.or over `threads` threads of barrier `id`.
 __device__ __forceinline__ bool bar_any(int id, int threads, bool v) {
     uint32_t r;
@@ -277,7 +283,6 @@ struct Kernel {
     static constexpr int kTop = BITS == 8 ? -3 : -7;
     static constexpr int NB = D / 64;                  // boxes of a K or V tile
     static constexpr int MB = D > 64 ? D / 128 : 1;    // 128-lane blocks of O^T (half used when d is 64)
-    static constexpr int kLoads = kQuant ? NB * BITS / 4 : 1;  // 16-byte loads of codes a producer thread makes per K or V tile
 
     __device__ static __forceinline__ Fixed& fixed() {
         extern __shared__ __align__(1024) uint8_t smem[];
@@ -410,16 +415,36 @@ struct Kernel {
         cp_async_wait_all();  // nothing is in flight when the block's shared memory goes
     }
 
-    // Quantised caches: codes to registers a tile ahead, unpacked to fp16 and stored swizzled.
-    __device__ static __forceinline__ void load_codes(const uint8_t* rows, int tile, int keys, int pt, uint4 (&r)[kLoads]) {
-        const int valid = keys - tile * kKeys;
-        const uint8_t* p = rows + (int64_t)(tile * kKeys + pt / kRowThreads) * (D * BITS / 8) + (pt % kRowThreads) * 16;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int b = i / kPieces, u = i % kPieces;
-            r[i] = piece_key(pt, u) < valid ? __ldcs(reinterpret_cast<const uint4*>(
-                                                  p + b * (8 * BITS) + u * (256 / kRowThreads) * (D * BITS / 8)))
-                                            : make_uint4(0, 0, 0, 0);
+    // Quantised caches: one lane copies runs of rows to the staging slots with bulk copies (a slot is 64
+    // rows of 8-bit or 128 rows of 4-bit codes), the producers unpack them to fp16 boxes.  Rows behind the
+    // last one stay whatever the slot held: their scale and bias are 0.
+    static constexpr int kStageRows = kQuant ? 512 / BITS : 64;
+    __device__ static void stage(const Args& a, Walker w) {
+        Unit u;
+        int slot = 0;
+        uint32_t phase = 0;
+        while (w.next(a, u)) {
+            const Source src(a, u);
+#pragma unroll 1
+            for (int step = 1; step <= 2 * src.n; ++step) {  // K0 K1 V0 K2 V1 .. V(n-1)
+                const bool is_v = step > 1 && (step == 2 * src.n || (step & 1));
+                const int i = is_v ? (step == 2 * src.n ? src.n - 1 : step / 2 - 1) : step / 2;
+                const int key_at = (src.t0 + i) * kKeys;
+#pragma unroll 1
+                for (int r0 = 0; r0 < kKeys; r0 += kStageRows) {
+                    wait(&fixed().unstaged[slot], phase ^ 1);
+                    const int rows = min(kStageRows, max(0, src.keys - key_at - r0));
+                    const uint32_t bytes = rows * (D * BITS / 8);
+                    mbar_arrive_expect_tx(&fixed().staged[slot], bytes);
+                    if (bytes)
+                        bulk_copy(smem_at(a.l.stage) + slot * (64 * D),
+                                  (is_v ? src.v : src.k) + (int64_t)(key_at + r0) * (D * BITS / 8), bytes, &fixed().staged[slot]);
+                    if (++slot == a.stages) {
+                        slot = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
         }
     }
     // Scales and biases of one key, as raw bf16 pairs.
@@ -476,8 +501,8 @@ struct Kernel {
                 }
             }
     }
-    // Unpacks one 16-byte piece (32 or 16 elements of one key and group) into its chunks of a box row.
-    __device__ static __forceinline__ void unpack(uint4 codes, uint32_t sb, uint32_t row, int key, int piece) {
+    // Unpacks one 16-byte piece (32 or 16 elements of one key and group) to its chunks of a box row.
+    __device__ static __forceinline__ void unpack(uint4 codes, uint32_t sb, uint32_t row, const uint32_t (&chunk)[kChunks]) {
         const uint32_t s2 = __byte_perm(sb, 0, 0x1010), b2 = __byte_perm(sb, 0, 0x3232);
         const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
         if constexpr (BITS == 4) {
@@ -485,51 +510,94 @@ struct Kernel {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t hi = w[i] >> 8;
-                sts128(row + (((4 * piece + i) ^ (key & 7)) << 4),
-                       make_uint4(fma_h2(w[i] & 0x000f000fu, s2, b2), fma_h2(w[i] & 0x00f000f0u, t2, b2),
-                                  fma_h2(hi & 0x000f000fu, s2, b2), fma_h2(hi & 0x00f000f0u, t2, b2)));
+                sts128(row + chunk[i], make_uint4(fma_h2(w[i] & 0x000f000fu, s2, b2), fma_h2(w[i] & 0x00f000f0u, t2, b2),
+                                                  fma_h2(hi & 0x000f000fu, s2, b2), fma_h2(hi & 0x00f000f0u, t2, b2)));
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                sts128(row + (((2 * piece + i) ^ (key & 7)) << 4),
-                       make_uint4(fma_h2(__byte_perm(w[2 * i], 0, 0x4140), s2, b2),
-                                  fma_h2(__byte_perm(w[2 * i], 0, 0x4342), s2, b2),
-                                  fma_h2(__byte_perm(w[2 * i + 1], 0, 0x4140), s2, b2),
-                                  fma_h2(__byte_perm(w[2 * i + 1], 0, 0x4342), s2, b2)));
+                sts128(row + chunk[i], make_uint4(fma_h2(__byte_perm(w[2 * i], 0, 0x4140), s2, b2),
+                                                  fma_h2(__byte_perm(w[2 * i], 0, 0x4342), s2, b2),
+                                                  fma_h2(__byte_perm(w[2 * i + 1], 0, 0x4140), s2, b2),
+                                                  fma_h2(__byte_perm(w[2 * i + 1], 0, 0x4342), s2, b2)));
         }
     }
 
     __device__ static void produce_quant(const Args& a, Walker w) {
         const int pt = threadIdx.x - 32 * kSoftmaxWarps, groups = D / a.cache.group;
-        const int key_of = pt & (kKeys - 1), piece = pt % kRowThreads;
+        const int key_of = pt & (kKeys - 1), piece = pt % kRowThreads, key0 = pt / kRowThreads;
         const bool does_v = pt >= kKeys;
         const uint32_t v_bytes = kKeys * groups * 4, tk = smem_at(kTables), tv = tk + v_bytes;
         const uint32_t ring_at = smem_at(a.l.ring);
         const int shift = 31 - __clz(a.cache.group);
-        Ring ring{0, 0};
-        // look: first row of the tile to look at for non-finite values, kKeys for none
-        const auto emit = [&](const uint4 (&r)[kLoads], uint32_t table, int look, int unit) {
+        // A quarter-warp reads the same columns of two (8 bits) or four (4 bits) rows, which would lie in the same
+        // banks: the rows take their boxes in another order each.
+        constexpr int kRowBytes = D * BITS / 8, kMix = kRowBytes >= 128 ? 8 / kRowThreads : kRowBytes == 64 && NB > 1 ? 2 : 1;
+        const int mix = (kRowBytes >= 128 ? key0 : key0 >> 1) & (kMix - 1);
+        uint32_t chunk[kChunks];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                wait(&fixed().empty[ring.slot], ring.phase ^ 1);
-                const uint32_t box = ring_at + ring.slot * kBox;
+        for (int i = 0; i < kChunks; ++i) chunk[i] = key0 * 128 + (((kChunks * piece + i) ^ (key0 & 7)) << 4);
+        const uint32_t from = smem_at(a.l.stage) + key0 * kRowBytes + piece * 16;
+        Ring ring{0, 0};
+        int slot = 0;
+        uint32_t phase = 0;
+        // look: first row of the tile to look at for non-finite values, kKeys for none
+        const auto emit = [&](uint32_t table, int look, int unit) {
+            uint32_t codes[kPieces];
+#pragma unroll
+            for (int u = 0; u < kPieces; ++u) {
+                codes[u] = from + slot * (64 * D);
+                wait(&fixed().staged[slot], phase);
+                if (++slot == a.stages) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+            }
+            const uint32_t entry = table + key0 * groups * 4;
+#pragma unroll
+            for (int b0 = 0; b0 < NB; b0 += kMix) {
+                int at[kMix];
+#pragma unroll
+                for (int b = 0; b < kMix; ++b) {
+                    at[b] = ring.slot;
+                    wait(&fixed().empty[ring.slot], ring.phase ^ 1);
+                    ring.step(a.slots);
+                }
+#pragma unroll
+                for (int b = 0; b < kMix; ++b) {
+                    const int mine = b ^ mix, box = b0 + mine;  // the box this thread's row takes now
+                    int slot_of = at[0];
+#pragma unroll
+                    for (int x = 1; x < kMix; ++x) slot_of = mine == x ? at[x] : slot_of;
+                    const uint32_t sb = entry + ((box * 64 + piece * (128 / BITS)) >> shift) * 4;
+#pragma unroll
+                    for (int u = 0; u < kPieces; ++u)
+                        unpack(lds128(codes[u] + box * (8 * BITS)), lds32(sb + u * (256 / kRowThreads) * groups * 4),
+                               ring_at + slot_of * kBox + u * (256 / kRowThreads) * 128, chunk);
+                }
+                if (__builtin_expect(look < kKeys, 0))
+#pragma unroll
+                    for (int b = 0; b < kMix; ++b)
+                        take_out(ring_at + at[b] * kBox, look, pt, &fixed().poison[unit & (kPoison - 1)]);
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+                    for (int b = 0; b < kMix; ++b) mbar_arrive(&fixed().full[at[b]]);
+                }
+            }
+            // the codes have been read
+            if ((threadIdx.x & 31) == 0) {
 #pragma unroll
                 for (int u = 0; u < kPieces; ++u) {
-                    const int key = piece_key(pt, u), group = (b * 64 + piece * (128 / BITS)) >> shift;
-                    unpack(r[b * kPieces + u], lds32(table + (key * groups + group) * 4), box + key * 128, key, piece);
+                    const int back = slot - kPieces + u;
+                    mbar_arrive(&fixed().unstaged[back < 0 ? back + a.stages : back]);
                 }
-                if (__builtin_expect(look < kKeys, 0)) take_out(box, look, pt, &fixed().poison[unit & (kPoison - 1)]);
-                signal_full(ring.slot);
-                ring.step(a.slots);
             }
         };
         Unit u;
         if (!w.next(a, u)) return;
         Source cur(a, u), next;
-        uint4 kr[kLoads], vr[kLoads];
         Groups g;
-        load_codes(cur.k, cur.t0, cur.keys, pt, kr);
         load_groups(a, cur, does_v, cur.t0 * kKeys + key_of, groups, g);
         int tile = 0;
         bool more = true;
@@ -556,18 +624,14 @@ struct Kernel {
                     }
                     named_bar_sync(3, 32 * kProducerWarps);
                     if (pt == 0) mbar_arrive(&fixed().sc_full[depth]);
-                    const bool last = i + 1 == cur.n;
-                    if (!last) load_groups(a, cur, does_v, (cur.t0 + i + 1) * kKeys + key_of, groups, g);
+                    if (i + 1 < cur.n) load_groups(a, cur, does_v, (cur.t0 + i + 1) * kKeys + key_of, groups, g);
                     else if (more) load_groups(a, next, does_v, next.t0 * kKeys + key_of, groups, g);
-                    emit(kr, tk, kKeys, 0);
-                    if (!last) load_codes(cur.k, cur.t0 + i + 1, cur.keys, pt, kr);
-                    else if (more) load_codes(next.k, next.t0, next.keys, pt, kr);
+                    emit(tk, kKeys, 0);
                 }
                 if (i > 0) {
                     const int at = (cur.t0 + i - 1) * kKeys, look = max(0, cur.hidden - at);
-                    emit(vr, tv + ((tile - 1) & 1) * v_bytes, at + look < cur.keys ? look : kKeys, unit);
+                    emit(tv + ((tile - 1) & 1) * v_bytes, at + look < cur.keys ? look : kKeys, unit);
                 }
-                if (i < cur.n) load_codes(cur.v, cur.t0 + i, cur.keys, pt, vr);
             }
             --tile;  // the unit's last pass was V alone
             cur = next;
@@ -979,6 +1043,10 @@ struct Kernel {
                 mbar_init(&fixed().sc_full[i], 1);
                 mbar_init(&fixed().sc_empty[i], kSoftmaxWarps);
             }
+            for (int i = 0; i < kMaxStages; ++i) {
+                mbar_init(&fixed().staged[i], 1);
+                mbar_init(&fixed().unstaged[i], kProducerWarps);
+            }
             fixed().abort = 0;
             fence_barrier_init();
         }
@@ -993,19 +1061,16 @@ struct Kernel {
         const uint32_t tmem = *reinterpret_cast<volatile int*>(&fixed().tmem);
         const Walker w{fixed().w0, fixed().w1, fixed().entry, fixed().off};
         if (warp < kSoftmaxWarps) {
-            if constexpr (!kQuant) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(120));
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             softmax(a, w, tmem, blockIdx.x);
         } else if (warp < kSoftmaxWarps + kProducerWarps) {
-            if constexpr (kQuant) {
-                asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(120));
-                produce_quant(a, w);
-            } else {
-                asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(72));
-                produce_bf16(a, w);
-            }
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+            if constexpr (kQuant) produce_quant(a, w);
+            else produce_bf16(a, w);
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
             if (warp == kSoftmaxWarps + kProducerWarps) issue(a, tmem);
+            else if (kQuant && threadIdx.x == 32 * (kSoftmaxWarps + kProducerWarps + 1)) stage(a, w);
             __syncwarp();
         }
         tc5::fence_before();
@@ -1162,9 +1227,17 @@ static size_t fit(Args& a, const dflash_kv_cache& c, int prefix_len, int tokens,
     a.rows_o = static_cast<int>(rows_o < kRows ? rows_o : kRows);
     a.nr = (prefix_len ? rows_p : rows_o) <= 64 ? 64 : kRows;
     const int groups = c.bits == 16 ? 0 : c.head_dim / c.group;
-    a.slots = kMaxSlots;
-    while (layout(c.head_dim, a.nr, a.slots, groups).total > kSmemLimit) a.slots -= 2;
-    a.l = layout(c.head_dim, a.nr, a.slots, groups);
+    // bf16: all that fits in ring slots.  Quantised: four staging slots or more (two K or V tiles of 8-bit codes)
+    // first, then ring slots, then the rest to staging; three where 128 query rows of 256 leave no more.
+    a.slots = c.bits == 16 ? kMaxSlots : 8;
+    a.stages = c.bits == 16 ? 0 : 4;
+    const auto fits = [&](int slots, int stages) {
+        return layout(c.head_dim, a.nr, slots, stages, groups).total <= kSmemLimit;
+    };
+    while (!fits(a.slots, a.stages) && a.slots > 4) a.slots -= 2;
+    while (!fits(a.slots, a.stages)) --a.stages;
+    while (c.bits != 16 && a.stages < kMaxStages && fits(a.slots, a.stages + 1)) ++a.stages;
+    a.l = layout(c.head_dim, a.nr, a.slots, a.stages, groups);
     size_t at = 0;
     const auto take = [&](size_t bytes) {
         uint8_t* p = base + at;
