@@ -95,7 +95,8 @@ struct Args {
     int prefix_len, tokens, hq;
     float scale;
     // sizes that follow from the above
-    int G, blocks_p, blocks_o;   // row blocks of the prefix and of one sequence
+    int G, g_magic;              // q heads per kv head, and 2^16 / G rounded up
+    int blocks_p, blocks_o;      // row blocks of the prefix and of one sequence
     int rows_o;                  // rows of a block of one sequence, at most
     int nr;                      // columns of the products' buffers: 64 or kRows
     int slots, stages;           // ring slots, staging slots (quantised caches)
@@ -266,7 +267,7 @@ __device__ __forceinline__ bool try_wait_1us(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(smem_u32(bar)), "r"(parity)
@@ -712,37 +713,50 @@ struct Kernel {
     // Q of a unit: rows of the block as K-major swizzled boxes; over quantised caches as fp16 scaled by a
     // power of two per row, in the order that the unpack leaves.
     __device__ static __forceinline__ void load_q(const Args& a, const Unit& u) {
-        constexpr int kPieces = D / 8;
+        constexpr int kPer = D / 8, kBatch = 4;  // 16-byte pieces of a row, which sit in one warp; loads in flight
         const int tid = threadIdx.x;
-        for (int idx = tid; idx < u.rows * kPieces; idx += 32 * kSoftmaxWarps) {
-            const int n = idx / kPieces, c = idx % kPieces;  // a row's pieces sit in one warp
-            const int r = u.block * kRows + n;
-            const int64_t row = u.prefix ? r / a.G : (int64_t)u.seq * a.tokens + r / a.G;
-            const uint4 x = *reinterpret_cast<const uint4*>(a.q + row * a.ld_q + (size_t)(u.head * a.G + r % a.G) * D + c * 8);
-            uint4 y = x;
-            if constexpr (kQuant) {
-                float f[8];
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                float m = 0.f;
+        const int t0 = u.block * kRows / a.G, g0 = u.block * kRows - t0 * a.G;
+        const uint16_t* base = a.q + ((u.prefix ? 0 : (int64_t)u.seq * a.tokens) + t0) * a.ld_q + (size_t)u.head * a.G * D;
+        // row n of the block is token t0 + v / G, head v % G of v = g0 + n < 256: a product with 2^16 / G
+        const auto token_of = [&](int n) { return static_cast<int>(static_cast<uint32_t>((g0 + n) * a.g_magic) >> 16); };
+        for (int first = 0; first < u.rows * kPer; first += 32 * kSoftmaxWarps * kBatch) {
+            uint4 x[kBatch];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    f[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-                    m = fmaxf(m, fabsf(f[i]));
+            for (int k = 0; k < kBatch; ++k) {
+                const int idx = first + k * 32 * kSoftmaxWarps + tid, n = idx / kPer, c = idx % kPer;
+                x[k] = make_uint4(0, 0, 0, 0);
+                if (n < u.rows) {
+                    const int t = token_of(n);
+                    x[k] = *reinterpret_cast<const uint4*>(base + t * a.ld_q + (g0 + n - t * a.G) * D + c * 8);
                 }
-                const uint32_t mask = __activemask();
-#pragma unroll
-                for (int o = 1; o < kPieces && o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, o));
-                const int e = min(max(exponent(m), -100), 120);
-                const float sc = exp2i(kTopQ - e);
-                uint32_t* p = &y.x;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] = pack2<false>(f[order<BITS>(2 * i)] * sc, f[order<BITS>(2 * i + 1)] * sc);
-                if (c == 0) fixed().qs[n] = a.scale * 1.4426950408889634f * exp2i(e - kTopQ);
             }
-            sts128(smem_at(a.l.q) + (c >> 3) * a.nr * 128 + n * 128 + (((c & 7) ^ (n & 7)) << 4), y);
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int idx = first + k * 32 * kSoftmaxWarps + tid, n = idx / kPer, c = idx % kPer;
+                uint4 y = x[k];
+                if constexpr (kQuant) {
+                    float f[8];
+                    const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+                    float m = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        f[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+                        m = fmaxf(m, fabsf(f[i]));
+                    }
+#pragma unroll
+                    for (int o = 1; o < kPer; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    const int e = min(max(exponent(m), -100), 120);
+                    const float sc = exp2i(kTopQ - e);
+                    uint32_t* p = &y.x;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[i] = pack2<false>(f[order<BITS>(2 * i)] * sc, f[order<BITS>(2 * i + 1)] * sc);
+                    if (c == 0 && n < u.rows) fixed().qs[n] = a.scale * 1.4426950408889634f * exp2i(e - kTopQ);
+                }
+                if (n < u.rows) sts128(smem_at(a.l.q) + (c >> 3) * a.nr * 128 + n * 128 + (((c & 7) ^ (n & 7)) << 4), y);
+            }
         }
         if (tid < kRows) {
-            const int n = tid, r = u.block * kRows + n;
+            const int n = tid;
             const bool live = n < u.rows;
             fixed().thr[n] = live ? -INFINITY : INFINITY;  // a row that is not there never raises its maximum
             fixed().mm[n] = -kLift;
@@ -750,7 +764,7 @@ struct Kernel {
             // key b of the block (below 0: cached rows) is seen if b <= info, in a tree if bit b of info is set
             int info = -1;
             if (live && !u.prefix) {
-                const int t = r / a.G;
+                const int t = t0 + token_of(n);
                 info = a.parents ? static_cast<int>(tree_walk(a.parents + (size_t)u.seq * a.tokens, t).path) : t;
             }
             fixed().info[n] = info;
@@ -1003,8 +1017,11 @@ struct Kernel {
         // with nothing but absent sequences the prefix has no reader
         if (total == prefix_end) total = 0;
         const int ctas = min(static_cast<int>(gridDim.x), total), cta = blockIdx.x;
-        const int w0 = cta < ctas ? static_cast<int>((long long)total * cta / ctas) : 0;
-        const int w1 = cta < ctas ? static_cast<int>((long long)total * (cta + 1) / ctas) : 0;
+        const auto share = [&](int c) {  // floor(total c / ctas)
+            return total < (1 << 23) ? static_cast<int>(static_cast<uint32_t>(total * c) / static_cast<uint32_t>(ctas))
+                                     : static_cast<int>((long long)total * c / ctas);
+        };
+        const int w0 = cta < ctas ? share(cta) : 0, w1 = cta < ctas ? share(cta + 1) : 0;
         const int w = max(w0, prefix_end);  // first own tile of the run
         if (tid == 0) {
             fixed().w0 = w0;
@@ -1221,6 +1238,7 @@ static size_t fit(Args& a, const dflash_kv_cache& c, int prefix_len, int tokens,
     a.tokens = tokens;
     a.hq = hq;
     a.G = hq / c.kv_heads;
+    a.g_magic = (65536 + a.G - 1) / a.G;  // v / G exactly for v < 256, G <= 64: v (G - 1) < 2^16
     const long long rows_p = (long long)c.sequences * tokens * a.G, rows_o = (long long)tokens * a.G;
     a.blocks_p = prefix_len ? static_cast<int>((rows_p + kRows - 1) / kRows) : 0;
     a.blocks_o = static_cast<int>((rows_o + kRows - 1) / kRows);
