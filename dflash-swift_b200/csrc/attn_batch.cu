@@ -21,7 +21,8 @@
 //
 // Roles: warps 0-7 softmax (two per TMEM lane quarter, half of the columns each), 8-15 producers
 // (cache rows to swizzled shared memory boxes of 128 keys x 64 elements, in a ring), warp 16 issues
-// the products, warp 17 the bulk copies of codes to staging slots (18 and 19 have no work).  The running maximum is only raised when a score passes it by kLazy (in powers
+// the products, warp 17 the bulk copies of codes to staging slots (18 and 19 have
+// no work).  The running maximum is only raised when a score passes it by kLazy (in powers
 // of two), so the accumulators are rarely rescaled.
 #include "common.cuh"
 #include "dflash_batch.h"
@@ -34,16 +35,16 @@ namespace attn {
 
 constexpr int kKeys = 128;
 constexpr int kRows = 128;
-constexpr int kBox = kKeys * 128;          // bytes of a ring slot: 128 keys x 64 elements of 16 bits
+constexpr int kBox = kKeys * 128;          // bytes of a box: 128 keys x 64 elements of 16 bits
 constexpr int kSoftmaxWarps = 8, kProducerWarps = 8;
 constexpr int kThreads = 32 * (kSoftmaxWarps + kProducerWarps + 4);  // whole warpgroups: registers move between them
 // Registers a thread.  The block starts with kThreads x 96 = 61440 and every warpgroup takes or gives; what is
 // taken is never more than what is given, so nobody waits for good: 256 x 112 + 256 x 80 + 128 x 72 = 58368.
 constexpr int kSoftmaxRegs = 112, kProducerRegs = 80, kIssueRegs = 72;
 constexpr int kMaxCtas = 160;              // partials are sized for this many CTAs
-constexpr int kMaxSlots = 10;
-constexpr int kMaxStages = 8;              // staging slots for codes, 64 d bytes each
-constexpr int kScaleDepth = 4;             // tiles whose key factors may be alive at once
+constexpr int kMaxSlots = 10;              // ring slots: two boxes each, one where d is 64
+constexpr int kMaxStages = 8;              // staging slots for codes: 64 or 128 rows each
+constexpr int kScaleDepth = 2;             // tiles whose key factors may be alive at once
 constexpr int kPoison = 16;                // units whose poison flags may be alive at once
 constexpr float kLazy = 4.f;               // a maximum moves when a score passes it by 2^4 ...
 constexpr float kLift = 8.f;               // ... and P is 2^8 p, up to 2^12: small weights stay normal in fp16
@@ -74,13 +75,13 @@ constexpr uint32_t kTables = (sizeof(Fixed) + 15) / 16 * 16;
 struct Layout {
     uint32_t ring, q, p, stage, total;
 };
-__host__ inline Layout layout(int d, int nr, int slots, int stages, int groups) {
+__host__ inline Layout layout(int d, int nr, int slots, int stages, int stage_bytes, int groups) {
     Layout l;
     l.ring = (kTables + 3 * kKeys * groups * 4 + 1023) / 1024 * 1024;
-    l.q = l.ring + slots * kBox;
+    l.q = l.ring + slots * (d > 64 ? 2 : 1) * kBox;
     l.p = l.q + nr * d * 2;
     l.stage = l.p + kKeys * nr * 2;
-    l.total = l.stage + stages * 64 * d;
+    l.total = l.stage + stages * stage_bytes;
     return l;
 }
 
@@ -99,7 +100,7 @@ struct Args {
     int blocks_p, blocks_o;      // row blocks of the prefix and of one sequence
     int rows_o;                  // rows of a block of one sequence, at most
     int nr;                      // columns of the products' buffers: 64 or kRows
-    int slots, stages;           // ring slots, staging slots (quantised caches)
+    int slots, stages, stage_rows;  // ring slots; staging slots and their rows (quantised caches)
     Layout l;
     // workspace: partials of the prefix, then of the sequences
     int32_t* first;              // [segments] first and last CTA of each (row block, kv head)
@@ -283,7 +284,8 @@ struct Kernel {
     // to stay under 2^-8 (store_groups).
     static constexpr int kTop = BITS == 8 ? -3 : -7;
     static constexpr int NB = D / 64;                  // boxes of a K or V tile
-    static constexpr int MB = D > 64 ? D / 128 : 1;    // 128-lane blocks of O^T (half used when d is 64)
+    static constexpr int MB = D > 64 ? D / 128 : 1;    // 128-lane blocks of O^T (half used when d is 64) = ring slots of a tile
+    static constexpr int kSub = NB / MB, kSlot = kSub * kBox;  // boxes and bytes of a ring slot
 
     __device__ static __forceinline__ Fixed& fixed() {
         extern __shared__ __align__(1024) uint8_t smem[];
@@ -395,16 +397,20 @@ struct Kernel {
                 const int look = max(0, src.hidden - key_at);
                 const uint8_t* p = (is_v ? src.v : src.k) + ((int64_t)(key_at + key0) * D + c * 8) * 2;
 #pragma unroll 1
-                for (int b = 0; b < NB; ++b, p += 128) {
+                for (int b = 0; b < MB; ++b, p += kSub * 128) {
                     wait(&fixed().empty[ring.slot], ring.phase ^ 1);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const bool live = key0 + 32 * x < valid;
-                        cp_async16(dst0 + ring.slot * kBox + x * 4096, live ? p + x * (32 * D * 2) : src.k, live);
+#pragma unroll
+                        for (int y = 0; y < kSub; ++y)
+                            cp_async16(dst0 + ring.slot * kSlot + y * kBox + x * 4096,
+                                       live ? p + x * (32 * D * 2) + y * 128 : src.k, live);
                     }
                     if (__builtin_expect(is_v && look < valid, 0)) {
                         cp_async_wait_all();
-                        take_out(ring_at + ring.slot * kBox, look, pt, &fixed().poison[unit & (kPoison - 1)]);
+                        for (int y = 0; y < kSub; ++y)
+                            take_out(ring_at + ring.slot * kSlot + y * kBox, look, pt, &fixed().poison[unit & (kPoison - 1)]);
                         mbar_arrive(&fixed().full[ring.slot]);
                     } else {
                         cp_async_arrive(&fixed().full[ring.slot]);
@@ -416,11 +422,11 @@ struct Kernel {
         cp_async_wait_all();  // nothing is in flight when the block's shared memory goes
     }
 
-    // Quantised caches: one lane copies runs of rows to the staging slots with bulk copies (a slot is 64
-    // rows of 8-bit or 128 rows of 4-bit codes), the producers unpack them to fp16 boxes.  Rows behind the
-    // last one stay whatever the slot held: their scale and bias are 0.
-    static constexpr int kStageRows = kQuant ? 512 / BITS : 64;
+    // Quantised caches: one lane copies runs of rows to the staging slots with bulk copies, the producers
+    // unpack the codes to fp16 boxes.  Rows behind the last one stay
+    // whatever the slot held: their scale and bias are 0.
     __device__ static void stage(const Args& a, Walker w) {
+        const uint32_t slot_bytes = a.stage_rows * (D * BITS / 8);
         Unit u;
         int slot = 0;
         uint32_t phase = 0;
@@ -432,13 +438,12 @@ struct Kernel {
                 const int i = is_v ? (step == 2 * src.n ? src.n - 1 : step / 2 - 1) : step / 2;
                 const int key_at = (src.t0 + i) * kKeys;
 #pragma unroll 1
-                for (int r0 = 0; r0 < kKeys; r0 += kStageRows) {
+                for (int r0 = 0; r0 < kKeys; r0 += a.stage_rows) {
                     wait(&fixed().unstaged[slot], phase ^ 1);
-                    const int rows = min(kStageRows, max(0, src.keys - key_at - r0));
-                    const uint32_t bytes = rows * (D * BITS / 8);
+                    const uint32_t bytes = min(a.stage_rows, max(0, src.keys - key_at - r0)) * (D * BITS / 8);
                     mbar_arrive_expect_tx(&fixed().staged[slot], bytes);
                     if (bytes)
-                        bulk_copy(smem_at(a.l.stage) + slot * (64 * D),
+                        bulk_copy(smem_at(a.l.stage) + slot * slot_bytes,
                                   (is_v ? src.v : src.k) + (int64_t)(key_at + r0) * (D * BITS / 8), bytes, &fixed().staged[slot]);
                     if (++slot == a.stages) {
                         slot = 0;
@@ -526,40 +531,52 @@ struct Kernel {
 
     __device__ static void produce_quant(const Args& a, Walker w) {
         const int pt = threadIdx.x - 32 * kSoftmaxWarps, groups = D / a.cache.group;
-        const int key_of = pt & (kKeys - 1), piece = pt % kRowThreads, key0 = pt / kRowThreads;
-        const bool does_v = pt >= kKeys;
-        const uint32_t v_bytes = kKeys * groups * 4, tk = smem_at(kTables), tv = tk + v_bytes;
-        const uint32_t ring_at = smem_at(a.l.ring);
+        const int piece = pt % kRowThreads, key0 = pt / kRowThreads;
+        const uint32_t ring_at = smem_at(a.l.ring), slot_bytes = a.stage_rows * (D * BITS / 8);
         const int shift = 31 - __clz(a.cache.group);
         // A quarter-warp reads the same columns of two (8 bits) or four (4 bits) rows, which would lie in the same
         // banks: the rows take their boxes in another order each.
         constexpr int kRowBytes = D * BITS / 8, kMix = kRowBytes >= 128 ? 8 / kRowThreads : kRowBytes == 64 && NB > 1 ? 2 : 1;
+        static_assert(kMix % kSub == 0, "whole ring slots at a time");
         const int mix = (kRowBytes >= 128 ? key0 : key0 >> 1) & (kMix - 1);
         uint32_t chunk[kChunks];
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) chunk[i] = key0 * 128 + (((kChunks * piece + i) ^ (key0 & 7)) << 4);
         const uint32_t from = smem_at(a.l.stage) + key0 * kRowBytes + piece * 16;
+        const bool halves = a.stage_rows < kKeys;
+        // Scales: a warp unpacks the same 16 keys of every tile, so it keeps their tables for itself; when it comes to a
+        // tile's K its lower lanes take the 16 keys of K, the upper ones those of V, whose factor the softmax needs
+        // before V is unpacked.
+        const int lane = threadIdx.x & 31, kk = lane & 15;
+        const bool does_v = lane >= 16;
+        const int key_of = (pt >> 5) * (BITS == 8 ? 8 : 16) + (BITS == 8 ? (kk & 7) + 64 * (kk >> 3) : kk);
+        const uint32_t v_bytes = kKeys * groups * 4, tk = smem_at(kTables), tv = tk + v_bytes;
+        Groups g;
         Ring ring{0, 0};
         int slot = 0;
         uint32_t phase = 0;
         // look: first row of the tile to look at for non-finite values, kKeys for none
         const auto emit = [&](uint32_t table, int look, int unit) {
-            uint32_t codes[kPieces];
+            uint32_t codes[kPieces];  // kPieces x (256 / kRowThreads) rows: one slot, or two halves
 #pragma unroll
-            for (int u = 0; u < kPieces; ++u) {
-                codes[u] = from + slot * (64 * D);
-                wait(&fixed().staged[slot], phase);
-                if (++slot == a.stages) {
-                    slot = 0;
-                    phase ^= 1;
+            for (int x = 0; x < kPieces; ++x) {
+                if (x == 0 || halves) {
+                    codes[x] = from + slot * slot_bytes;
+                    wait(&fixed().staged[slot], phase);
+                    if (++slot == a.stages) {
+                        slot = 0;
+                        phase ^= 1;
+                    }
+                } else {
+                    codes[x] = codes[0] + x * (256 / kRowThreads) * kRowBytes;
                 }
             }
             const uint32_t entry = table + key0 * groups * 4;
 #pragma unroll
             for (int b0 = 0; b0 < NB; b0 += kMix) {
-                int at[kMix];
+                int at[kMix / kSub];
 #pragma unroll
-                for (int b = 0; b < kMix; ++b) {
+                for (int b = 0; b < kMix / kSub; ++b) {
                     at[b] = ring.slot;
                     wait(&fixed().empty[ring.slot], ring.phase ^ 1);
                     ring.step(a.slots);
@@ -567,38 +584,35 @@ struct Kernel {
 #pragma unroll
                 for (int b = 0; b < kMix; ++b) {
                     const int mine = b ^ mix, box = b0 + mine;  // the box this thread's row takes now
-                    int slot_of = at[0];
-#pragma unroll
-                    for (int x = 1; x < kMix; ++x) slot_of = mine == x ? at[x] : slot_of;
+                    uint32_t row = at[0];
+                    if (kMix / kSub > 1) row = mine / kSub ? at[kMix / kSub - 1] : at[0];
+                    row = ring_at + row * kSlot + (mine % kSub) * kBox;
                     const uint32_t sb = entry + ((box * 64 + piece * (128 / BITS)) >> shift) * 4;
 #pragma unroll
-                    for (int u = 0; u < kPieces; ++u)
-                        unpack(lds128(codes[u] + box * (8 * BITS)), lds32(sb + u * (256 / kRowThreads) * groups * 4),
-                               ring_at + slot_of * kBox + u * (256 / kRowThreads) * 128, chunk);
+                    for (int x = 0; x < kPieces; ++x)
+                        unpack(lds128(codes[x] + box * (8 * BITS)), lds32(sb + x * (256 / kRowThreads) * groups * 4),
+                               row + x * (256 / kRowThreads) * 128, chunk);
                 }
                 if (__builtin_expect(look < kKeys, 0))
 #pragma unroll
                     for (int b = 0; b < kMix; ++b)
-                        take_out(ring_at + at[b] * kBox, look, pt, &fixed().poison[unit & (kPoison - 1)]);
+                        take_out(ring_at + at[b / kSub] * kSlot + (b % kSub) * kBox, look, pt,
+                                 &fixed().poison[unit & (kPoison - 1)]);
                 __syncwarp();
                 if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-                    for (int b = 0; b < kMix; ++b) mbar_arrive(&fixed().full[at[b]]);
+                    for (int b = 0; b < kMix / kSub; ++b) mbar_arrive(&fixed().full[at[b]]);
                 }
             }
-            // the codes have been read
-            if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-                for (int u = 0; u < kPieces; ++u) {
-                    const int back = slot - kPieces + u;
-                    mbar_arrive(&fixed().unstaged[back < 0 ? back + a.stages : back]);
-                }
+            if ((threadIdx.x & 31) == 0) {  // the codes have been read
+                const int last = slot == 0 ? a.stages - 1 : slot - 1;
+                mbar_arrive(&fixed().unstaged[last]);
+                if (halves) mbar_arrive(&fixed().unstaged[last == 0 ? a.stages - 1 : last - 1]);
             }
         };
         Unit u;
         if (!w.next(a, u)) return;
         Source cur(a, u), next;
-        Groups g;
         load_groups(a, cur, does_v, cur.t0 * kKeys + key_of, groups, g);
         int tile = 0;
         bool more = true;
@@ -608,10 +622,8 @@ struct Kernel {
 #pragma unroll 1
             for (int i = 0; i <= cur.n; ++i, ++tile) {
                 if (i < cur.n) {
-                    // key factors of this tile: K's by the lower 128 threads, V's by the upper ones
                     const int depth = tile % kScaleDepth;
                     wait(&fixed().sc_empty[depth], ((tile / kScaleDepth) & 1) ^ 1);
-                    named_bar_sync(3, 32 * kProducerWarps);  // every thread is done with the tables that are rewritten
                     const float top = largest(g, groups);
                     if (does_v) {
                         const int e = min(max(exponent(top), -15), 24);
@@ -623,8 +635,8 @@ struct Kernel {
                         store_groups(tk + key_of * groups * 4, g, groups, exp2i(kTop - e));
                         fixed().key_k[depth][key_of] = exp2i(e - kTop);
                     }
-                    named_bar_sync(3, 32 * kProducerWarps);
-                    if (pt == 0) mbar_arrive(&fixed().sc_full[depth]);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&fixed().sc_full[depth]);
                     if (i + 1 < cur.n) load_groups(a, cur, does_v, (cur.t0 + i + 1) * kKeys + key_of, groups, g);
                     else if (more) load_groups(a, next, does_v, next.t0 * kKeys + key_of, groups, g);
                     emit(tk, kKeys, 0);
@@ -660,14 +672,18 @@ struct Kernel {
             const auto scores = [&](int i) {
                 const uint32_t d = tmem + ((tile + i) & 1) * a.nr;
 #pragma unroll 1
-                for (int b = 0; b < NB; ++b) {
+                for (int b = 0; b < MB; ++b) {
                     wait(&fixed().full[ring.slot], ring.phase);
                     fence_proxy_async_shared();
-                    const uint32_t k = smem_at(a.l.ring) + ring.slot * kBox, qb = q + b * a.nr * 128;
+                    const uint32_t k = smem_at(a.l.ring) + ring.slot * kSlot, qb = q + b * kSub * a.nr * 128;
                     const uint64_t dk = tc5::operand(k, 16, 1024), dq = tc5::operand(qb, 16, 1024);
+                    const uint32_t q_step = a.nr * 128 / 16;
                     if (one) {
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) tc5::mma(d, dk + ks * 2, dq + ks * 2, desc_qk, b + ks > 0);  // 32 bytes on
+                        for (int y = 0; y < kSub; ++y)
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks)  // 32 bytes on
+                                tc5::mma(d, dk + y * (kBox / 16) + ks * 2, dq + y * q_step + ks * 2, desc_qk, b + y + ks > 0);
                         tc5::commit(&fixed().empty[ring.slot]);
                     }
                     ring.step(a.slots);
@@ -683,16 +699,10 @@ struct Kernel {
 #pragma unroll 1
                 for (int mb = 0; mb < MB; ++mb) {
                     const int slot = ring.slot;
-                    int slot2 = slot;
                     wait(&fixed().full[slot], ring.phase);
                     ring.step(a.slots);
-                    if (D > 64) {
-                        slot2 = ring.slot;
-                        wait(&fixed().full[slot2], ring.phase);
-                        ring.step(a.slots);
-                    }
                     fence_proxy_async_shared();
-                    const uint64_t dv = tc5::operand(smem_at(a.l.ring) + slot * kBox, kBox, 1024);
+                    const uint64_t dv = tc5::operand(smem_at(a.l.ring) + slot * kSlot, kBox, 1024);
                     const uint64_t dp = tc5::operand(p, kBox, 1024);
                     const uint32_t d = tmem + (2 + mb) * a.nr;
                     if (one) {
@@ -700,7 +710,6 @@ struct Kernel {
                         for (int ks = 0; ks < kKeys / 16; ++ks)  // 16 keys of 128 bytes on
                             tc5::mma(d, dv + ks * 128, dp + ks * 128, desc_pv, i + ks > 0);
                         tc5::commit(&fixed().empty[slot]);
-                        if (D > 64) tc5::commit(&fixed().empty[slot2]);
                     }
                 }
                 if (one) tc5::commit(&fixed().pv_done);
@@ -1057,7 +1066,7 @@ struct Kernel {
             mbar_init(&fixed().pv_done, 1);
             mbar_init(&fixed().q_full, 1);
             for (int i = 0; i < kScaleDepth; ++i) {
-                mbar_init(&fixed().sc_full[i], 1);
+                mbar_init(&fixed().sc_full[i], kProducerWarps);
                 mbar_init(&fixed().sc_empty[i], kSoftmaxWarps);
             }
             for (int i = 0; i < kMaxStages; ++i) {
@@ -1245,17 +1254,19 @@ static size_t fit(Args& a, const dflash_kv_cache& c, int prefix_len, int tokens,
     a.rows_o = static_cast<int>(rows_o < kRows ? rows_o : kRows);
     a.nr = (prefix_len ? rows_p : rows_o) <= 64 ? 64 : kRows;
     const int groups = c.bits == 16 ? 0 : c.head_dim / c.group;
-    // bf16: all that fits in ring slots.  Quantised: four staging slots or more (two K or V tiles of 8-bit codes)
-    // first, then ring slots, then the rest to staging; three where 128 query rows of 256 leave no more.
-    a.slots = c.bits == 16 ? kMaxSlots : 8;
-    a.stages = c.bits == 16 ? 0 : 4;
+    // bf16: all that fits in ring slots.  Quantised: ring slots for a K or V tile and a half, then staging slots of
+    // whole tiles; of half tiles where two whole ones do not fit, and then fewer ring slots.
+    const int quant = c.bits != 16, sub = c.head_dim > 64 ? 2 : 1, row_bytes = c.head_dim * c.bits / 8;
+    a.stage_rows = kKeys;
     const auto fits = [&](int slots, int stages) {
-        return layout(c.head_dim, a.nr, slots, stages, groups).total <= kSmemLimit;
+        return layout(c.head_dim, a.nr, slots, stages, a.stage_rows * row_bytes, groups).total <= kSmemLimit;
     };
-    while (!fits(a.slots, a.stages) && a.slots > 4) a.slots -= 2;
-    while (!fits(a.slots, a.stages)) --a.stages;
-    while (c.bits != 16 && a.stages < kMaxStages && fits(a.slots, a.stages + 1)) ++a.stages;
-    a.l = layout(c.head_dim, a.nr, a.slots, a.stages, groups);
+    a.stages = quant ? 2 : 0;
+    a.slots = quant ? (c.head_dim == 256 ? 3 : 4) : kMaxSlots / sub;
+    if (c.bits == 8 && !fits(a.slots, 2)) a.stage_rows = kKeys / 2;
+    while (!fits(a.slots, a.stages)) --a.slots;
+    while (quant && a.stages < kMaxStages && fits(a.slots, a.stages + 1)) ++a.stages;
+    a.l = layout(c.head_dim, a.nr, a.slots, a.stages, a.stage_rows * row_bytes, groups);
     size_t at = 0;
     const auto take = [&](size_t bytes) {
         uint8_t* p = base + at;
