@@ -19,10 +19,10 @@
 // key's values (and every query row) are first scaled by a power of two into fp16's upper range,
 // undone in S^T for K and Q, and for V folded into P's exponent and the sum's weights.
 //
-// Roles: warps 0-7 softmax (two per TMEM lane quarter, half of the columns each), 8-15 producers
-// (cache rows to swizzled shared memory boxes of 128 keys x 64 elements, in a ring), warp 16 issues
-// the products, warp 17 the bulk copies of codes to staging slots (18 and 19 have
-// no work).  The running maximum is only raised when a score passes it by kLazy (in powers
+// Roles: warps 0-7 softmax (two per TMEM lane quarter, half of the columns each), 8-15 producers of K
+// and 16-23 of V (cache rows to swizzled shared memory boxes of 128 keys x 64 elements, in a ring),
+// warp 24 issues the products, warps 25 and 26 the bulk copies of K's and V's codes to staging
+// slots (27 has no work).  The running maximum is only raised when a score passes it by kLazy (in powers
 // of two), so the accumulators are rarely rescaled.
 #include "common.cuh"
 #include "dflash_batch.h"
@@ -36,11 +36,12 @@ namespace attn {
 constexpr int kKeys = 128;
 constexpr int kRows = 128;
 constexpr int kBox = kKeys * 128;          // bytes of a box: 128 keys x 64 elements of 16 bits
-constexpr int kSoftmaxWarps = 8, kProducerWarps = 8;
-constexpr int kThreads = 32 * (kSoftmaxWarps + kProducerWarps + 4);  // whole warpgroups: registers move between them
-// Registers a thread.  The block starts with kThreads x 96 = 61440 and every warpgroup takes or gives; what is
-// taken is never more than what is given, so nobody waits for good: 256 x 112 + 256 x 80 + 128 x 72 = 58368.
-constexpr int kSoftmaxRegs = 112, kProducerRegs = 80, kIssueRegs = 72;
+constexpr int kSoftmaxWarps = 8, kProducerWarps = 8;  // producers: this many for K and as many for V
+constexpr int kIssueWarp = kSoftmaxWarps + 2 * kProducerWarps;
+constexpr int kThreads = 32 * (kIssueWarp + 4);  // whole warpgroups: registers move between them
+// Registers a thread.  The block starts with kThreads x 72 = 64512; the issuing warpgroup gives 32 x 128 = 4096 and the
+// softmax takes 16 x 256 = 4096, so nobody waits for good.  The producers keep theirs.
+constexpr int kSoftmaxRegs = 88, kIssueRegs = 40;
 constexpr int kMaxCtas = 160;              // partials are sized for this many CTAs
 constexpr int kMaxSlots = 10;              // ring slots: two boxes each, one where d is 64
 constexpr int kMaxStages = 8;              // staging slots for codes: 64 or 128 rows each
@@ -62,14 +63,13 @@ struct Fixed {
     int info[kRows];                    // chain: the row's token; tree: its path mask
     float part[4][kRows];
     float key_k[kScaleDepth][kKeys], key_v[kScaleDepth][kKeys];
-    uint16_t key_w[kScaleDepth][kKeys];
     int poison[kPoison];
     int abort, tmem, w0, w1, entry, off;
     int unit_tiles, unit_rows;          // for the issuing thread, from the softmax warps
     int warp_sum[kThreads / 32];
 };
 static_assert(offsetof(Fixed, thr) % 16 == 0 && offsetof(Fixed, mm) % 16 == 0 && offsetof(Fixed, qs) % 16 == 0 &&
-                  offsetof(Fixed, key_w) % 4 == 0 && alignof(Fixed) == 16, "vector accesses");
+                  alignof(Fixed) == 16, "vector accesses");
 constexpr uint32_t kTables = (sizeof(Fixed) + 15) / 16 * 16;
 
 struct Layout {
@@ -99,8 +99,10 @@ struct Args {
     int G, g_magic;              // q heads per kv head, and 2^16 / G rounded up
     int blocks_p, blocks_o;      // row blocks of the prefix and of one sequence
     int rows_o;                  // rows of a block of one sequence, at most
+    int rb;                      // query rows of a block: kRows or 64
     int nr;                      // columns of the products' buffers: 64 or kRows
-    int slots, stages, stage_rows;  // ring slots; staging slots and their rows (quantised caches)
+    int slots_k, slots;          // ring slots: K's and all of them (quantised caches; one ring over bf16 caches)
+    int stages, stage_rows;      // staging slots of K, as many of V, and their rows (quantised caches)
     Layout l;
     // workspace: partials of the prefix, then of the sequences
     int32_t* first;              // [segments] first and last CTA of each (row block, kv head)
@@ -120,7 +122,7 @@ __host__ __device__ inline long long partials_p(const Args& a) { return a.blocks
 __host__ __device__ inline long long partials_o(const Args& a) { return segments_o(a) + kMaxCtas; }
 // Index of row 0 of a partial in ml (and, times d, in o).
 __device__ __forceinline__ long long partial_row(const Args& a, bool prefix, long long segment, int cta) {
-    return prefix ? (segment + cta) * kRows : partials_p(a) * kRows + (segment + cta) * a.rows_o;
+    return prefix ? (segment + cta) * a.rb : partials_p(a) * a.rb + (segment + cta) * a.rows_o;
 }
 __device__ __forceinline__ long long partial_index(const Args& a, bool prefix, long long segment, int cta) {
     return prefix ? segment + cta : partials_p(a) + segment + cta;
@@ -140,7 +142,7 @@ struct Unit {
 };
 
 __device__ __forceinline__ int own_keys(const Args& a, int len, int block) {
-    const int last = min(a.tokens * a.G, (block + 1) * kRows) - 1;
+    const int last = min(a.tokens * a.G, (block + 1) * a.rb) - 1;
     return a.parents ? len + a.tokens : len + last / a.G + 1;
 }
 __device__ __forceinline__ int live_length(const Args& a, int seq) {
@@ -167,7 +169,7 @@ struct Walker {
             u.seq = 0;
             u.tiles = tiles_p;
             u.t0 = w - s * tiles_p;
-            u.rows = min(kRows, a.cache.sequences * a.tokens * a.G - u.block * kRows);
+            u.rows = min(a.rb, a.cache.sequences * a.tokens * a.G - u.block * a.rb);
             u.len = u.keys = a.prefix_len;
         } else {
             int tiles = entry_tiles(a, entry);
@@ -183,7 +185,7 @@ struct Walker {
             u.segment = (long long)entry * a.cache.hkv + u.head;
             u.tiles = tiles;
             u.t0 = rel - u.head * tiles;
-            u.rows = min(kRows, a.tokens * a.G - u.block * kRows);
+            u.rows = min(a.rb, a.tokens * a.G - u.block * a.rb);
             u.len = a.lengths[u.seq];
             u.keys = own_keys(a, u.len, u.block);
         }
@@ -264,18 +266,6 @@ __device__ __forceinline__ int order(int i) {
     return BITS == 4 ? (i >> 1) + 4 * (i & 1) : i;
 }
 
-__device__ __forceinline__ bool try_wait_1us(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
 // ---------------------------------------------------------------- the kernel
 template <int BITS, int D>
 struct Kernel {
@@ -293,14 +283,15 @@ struct Kernel {
     }
     __device__ static __forceinline__ uint32_t smem_at(uint32_t offset) { return smem_u32(&fixed()) + offset; }
 
-    // A bounded wait that stays small where it is inlined: a failed try sleeps up to a microsecond, and
-    // 2^20 of them (a second at most) raise the error.  No clock is read, whose read costs more than the
-    // usual wait.  After an error every wait returns at once and the roles run on to their ends.
+    // A bounded wait that stays small where it is inlined: a failed try sleeps for as long as the hardware
+    // lets it (the phase's end wakes it), and 2^22 of them raise the error.  No clock is read, whose read
+    // costs more than the usual wait.  After an error every wait returns at once and the roles run on to
+    // their ends.
     __device__ static __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
         if (mbar_try_wait(bar, parity)) return;
-        for (int n = 0; !try_wait_1us(bar, parity); ++n) {
+        for (int n = 0; !mbar_try_wait(bar, parity); ++n) {
             if (*const_cast<volatile int*>(&fixed().abort)) return;
-            if (n == 1 << 20) {
+            if (n == 1 << 22) {
                 atomicOr(&g_device_error, DFLASH_DEVERR_ATTN_PIPELINE);
                 *const_cast<volatile int*>(&fixed().abort) = 1;
             }
@@ -308,18 +299,23 @@ struct Kernel {
     }
 
     // ------------------------------------------------------------ producers
-    // Boxes are produced in the order in which the products take them: in each unit K(0), then K(i)
-    // V(i - 1), then V(n - 1).
+    // The products take K(0), then K(i) V(i - 1), then V(n - 1) of a unit.
     struct Ring {
-        int slot;
+        int slot, first, end;
         uint32_t phase;
-        __device__ __forceinline__ void step(int slots) {
-            if (++slot == slots) {
-                slot = 0;
+        __device__ __forceinline__ void step() {
+            if (++slot == end) {
+                slot = first;
                 phase ^= 1;
             }
         }
     };
+    // K's and V's ring: one ring for both over bf16 caches, whose producers fill it in the products' order; one each
+    // where two groups of producers fill them, since a wait by parity only tells a phase from the one before it
+    // and a group must not run ahead of the other's use of a slot.
+    __device__ static __forceinline__ Ring ring_of(const Args& a, bool is_v) {
+        return kQuant && is_v ? Ring{a.slots_k, a.slots_k, a.slots, 0} : Ring{0, 0, a.slots_k, 0};
+    }
 
     // Where the rows of a unit's (sequence, kv head) lie.
     struct Source {
@@ -351,9 +347,10 @@ struct Kernel {
     }
 
     // The pieces of a box that a producer thread writes: kPieces rows, kChunks 16-byte chunks of each.
-    static constexpr int kPieces = kQuant ? BITS / 4 : 4, kChunks = kQuant ? 16 / BITS : 1;
+    static constexpr int kGroup = kQuant ? 32 * kProducerWarps : 64 * kProducerWarps;  // threads that fill a box
+    static constexpr int kPieces = kQuant ? BITS / 4 : 2, kChunks = kQuant ? 16 / BITS : 1;
     static constexpr int kRowThreads = kQuant ? BITS / 2 : 8;  // threads that share a row
-    __device__ static __forceinline__ int piece_key(int pt, int u) { return pt / kRowThreads + u * (256 / kRowThreads); }
+    __device__ static __forceinline__ int piece_key(int pt, int u) { return pt / kRowThreads + u * (kGroup / kRowThreads); }
 
     // A non-finite element of a row that some query row does not see would reach it as 0 * inf: it is
     // taken out of the operand and the unit's flag raised, for the join to put it back where it is
@@ -385,7 +382,7 @@ struct Kernel {
     __device__ static void produce_bf16(const Args& a, Walker w) {
         const int pt = threadIdx.x - 32 * kSoftmaxWarps, key0 = pt >> 3, c = pt & 7;
         const uint32_t ring_at = smem_at(a.l.ring), dst0 = ring_at + key0 * 128 + ((c ^ (key0 & 7)) << 4);
-        Ring ring{0, 0};
+        Ring ring = ring_of(a, false);
         Unit u;
         for (int unit = 0; w.next(a, u); ++unit) {
             const Source src(a, u);
@@ -400,12 +397,12 @@ struct Kernel {
                 for (int b = 0; b < MB; ++b, p += kSub * 128) {
                     wait(&fixed().empty[ring.slot], ring.phase ^ 1);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const bool live = key0 + 32 * x < valid;
+                    for (int x = 0; x < kPieces; ++x) {
+                        const bool live = key0 + 64 * x < valid;
 #pragma unroll
                         for (int y = 0; y < kSub; ++y)
-                            cp_async16(dst0 + ring.slot * kSlot + y * kBox + x * 4096,
-                                       live ? p + x * (32 * D * 2) + y * 128 : src.k, live);
+                            cp_async16(dst0 + ring.slot * kSlot + y * kBox + x * 64 * 128,
+                                       live ? p + x * (64 * D * 2) + y * 128 : src.k, live);
                     }
                     if (__builtin_expect(is_v && look < valid, 0)) {
                         cp_async_wait_all();
@@ -415,95 +412,98 @@ struct Kernel {
                     } else {
                         cp_async_arrive(&fixed().full[ring.slot]);
                     }
-                    ring.step(a.slots);
+                    ring.step();
                 }
             }
         }
         cp_async_wait_all();  // nothing is in flight when the block's shared memory goes
     }
 
-    // Quantised caches: one lane copies runs of rows to the staging slots with bulk copies, the producers
-    // unpack the codes to fp16 boxes.  Rows behind the last one stay
-    // whatever the slot held: their scale and bias are 0.
-    __device__ static void stage(const Args& a, Walker w) {
+    // Quantised caches: a lane each for K and V copies runs of rows to their staging slots with bulk copies, a
+    // group of producers each unpacks the codes to fp16 boxes.  Rows behind the last one stay whatever
+    // the slot held: their scale and bias are 0.
+    __device__ static void stage(const Args& a, Walker w, bool is_v) {
         const uint32_t slot_bytes = a.stage_rows * (D * BITS / 8);
+        const int first = is_v ? a.stages : 0;
         Unit u;
-        int slot = 0;
+        int slot = first;
         uint32_t phase = 0;
         while (w.next(a, u)) {
             const Source src(a, u);
+            const uint8_t* rows = is_v ? src.v : src.k;
 #pragma unroll 1
-            for (int step = 1; step <= 2 * src.n; ++step) {  // K0 K1 V0 K2 V1 .. V(n-1)
-                const bool is_v = step > 1 && (step == 2 * src.n || (step & 1));
-                const int i = is_v ? (step == 2 * src.n ? src.n - 1 : step / 2 - 1) : step / 2;
-                const int key_at = (src.t0 + i) * kKeys;
-#pragma unroll 1
-                for (int r0 = 0; r0 < kKeys; r0 += a.stage_rows) {
-                    wait(&fixed().unstaged[slot], phase ^ 1);
-                    const uint32_t bytes = min(a.stage_rows, max(0, src.keys - key_at - r0)) * (D * BITS / 8);
-                    mbar_arrive_expect_tx(&fixed().staged[slot], bytes);
-                    if (bytes)
-                        bulk_copy(smem_at(a.l.stage) + slot * slot_bytes,
-                                  (is_v ? src.v : src.k) + (int64_t)(key_at + r0) * (D * BITS / 8), bytes, &fixed().staged[slot]);
-                    if (++slot == a.stages) {
-                        slot = 0;
-                        phase ^= 1;
-                    }
+            for (int at = src.t0 * kKeys; at < (src.t0 + src.n) * kKeys; at += a.stage_rows) {
+                wait(&fixed().unstaged[slot], phase ^ 1);
+                const uint32_t bytes = min(a.stage_rows, max(0, src.keys - at)) * (D * BITS / 8);
+                mbar_arrive_expect_tx(&fixed().staged[slot], bytes);
+                if (bytes)
+                    bulk_copy(smem_at(a.l.stage) + slot * slot_bytes, rows + (int64_t)at * (D * BITS / 8), bytes,
+                              &fixed().staged[slot]);
+                if (++slot == first + a.stages) {
+                    slot = first;
+                    phase ^= 1;
                 }
             }
         }
     }
-    // Scales and biases of one key, as raw bf16 pairs.
+
+    // Scales and biases of one key, as raw bf16 pairs: up to two words of each, of four, for one lane.
     struct Groups {
-        uint32_t s[4], b[4];
+        uint32_t s[2], b[2];
     };
     __device__ static __forceinline__ void load_groups(const Args& a, const Source& src, bool is_v, int key, int groups,
-                                                       Groups& g) {
+                                                       int first, Groups& g) {
         const kv::View& c = src.prefix ? a.prefix : a.cache;
         const int64_t at = (src.row0 + key) * groups;
         const uint16_t *ps = (is_v ? c.vs : c.ks) + at, *pb = (is_v ? c.vb : c.kb) + at;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) g.s[i] = g.b[i] = 0;
+        for (int i = 0; i < 2; ++i) g.s[i] = g.b[i] = 0;
         if (key >= src.keys) return;
         if (groups == 1) {
-            g.s[0] = *ps;
-            g.b[0] = *pb;
+            if (first == 0) {
+                g.s[0] = *ps;
+                g.b[0] = *pb;
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (2 * i < groups) {
-                    g.s[i] = reinterpret_cast<const uint32_t*>(ps)[i];
-                    g.b[i] = reinterpret_cast<const uint32_t*>(pb)[i];
+            for (int i = 0; i < 2; ++i)
+                if (2 * (first + i) < groups && (i == 0 || groups == 8)) {
+                    g.s[i] = reinterpret_cast<const uint32_t*>(ps)[first + i];
+                    g.b[i] = reinterpret_cast<const uint32_t*>(pb)[first + i];
                 }
         }
     }
-    // Largest magnitude that a key's groups can stand for.
-    __device__ static __forceinline__ float largest(const Groups& g, int groups) {
+    // Largest magnitude that a lane's groups can stand for.
+    __device__ static __forceinline__ float largest(const Groups& g) {
         constexpr float kCodes = BITS == 8 ? 255.f : 15.f;
         float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (2 * i < groups) {
-                const float s0 = __uint_as_float(g.s[i] << 16), s1 = __uint_as_float(g.s[i] & 0xffff0000u);
-                const float b0 = __uint_as_float(g.b[i] << 16), b1 = __uint_as_float(g.b[i] & 0xffff0000u);
-                m = fmaxf(m, fmaxf(fabsf(b0), fabsf(fmaf(kCodes, s0, b0))));
-                m = fmaxf(m, fmaxf(fabsf(b1), fabsf(fmaf(kCodes, s1, b1))));  // zero where groups is 1
-            }
+        for (int i = 0; i < 2; ++i) {  // zero where there is none
+            const float s0 = __uint_as_float(g.s[i] << 16), s1 = __uint_as_float(g.s[i] & 0xffff0000u);
+            const float b0 = __uint_as_float(g.b[i] << 16), b1 = __uint_as_float(g.b[i] & 0xffff0000u);
+            m = largest_of(m, b0, fmaf(kCodes, s0, b0));
+            m = largest_of(m, b1, fmaf(kCodes, s1, b1));
+        }
+        return m;
+    }
+    __device__ static __forceinline__ float largest_of(float m, float x, float y) {  // NaN stays NaN
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(x)));
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(fabsf(y)));
         return m;
     }
     // Table entries (fp16 scale * f * 2^24, bias * f): a code in the low bits of a half is the subnormal
     // code * 2^-24, so that one fma gives scale * code + bias (|scale * f| < 2^-8: see kTop).
-    __device__ static __forceinline__ void store_groups(uint32_t addr, const Groups& g, int groups, float f) {
+    __device__ static __forceinline__ void store_groups(uint32_t addr, const Groups& g, int groups, int first, float f) {
         const float f24 = f * 16777216.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (2 * i < groups) {
+        for (int i = 0; i < 2; ++i)
+            if (2 * (first + i) < groups && (i == 0 || groups == 8)) {
                 const uint32_t e0 = pack2<false>(__uint_as_float(g.s[i] << 16) * f24, __uint_as_float(g.b[i] << 16) * f);
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr + 8 * i), "r"(e0) : "memory");
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr + 8 * (first + i)), "r"(e0) : "memory");
                 if (groups > 1) {
                     const uint32_t e1 = pack2<false>(__uint_as_float(g.s[i] & 0xffff0000u) * f24,
                                                      __uint_as_float(g.b[i] & 0xffff0000u) * f);
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr + 8 * i + 4), "r"(e1) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr + 8 * (first + i) + 4), "r"(e1) : "memory");
                 }
             }
     }
@@ -529,121 +529,111 @@ struct Kernel {
         }
     }
 
-    __device__ static void produce_quant(const Args& a, Walker w) {
-        const int pt = threadIdx.x - 32 * kSoftmaxWarps, groups = D / a.cache.group;
+    __device__ static void produce_quant(const Args& a, Walker w, bool is_v) {
+        const int pt = threadIdx.x & (32 * kProducerWarps - 1), groups = D / a.cache.group;
         const int piece = pt % kRowThreads, key0 = pt / kRowThreads;
         const uint32_t ring_at = smem_at(a.l.ring), slot_bytes = a.stage_rows * (D * BITS / 8);
         const int shift = 31 - __clz(a.cache.group);
         // A quarter-warp reads the same columns of two (8 bits) or four (4 bits) rows, which would lie in the same
-        // banks: the rows take their boxes in another order each.
-        constexpr int kRowBytes = D * BITS / 8, kMix = kRowBytes >= 128 ? 8 / kRowThreads : kRowBytes == 64 && NB > 1 ? 2 : 1;
-        static_assert(kMix % kSub == 0, "whole ring slots at a time");
-        const int mix = (kRowBytes >= 128 ? key0 : key0 >> 1) & (kMix - 1);
+        // banks: every other row takes the two boxes of a slot in the other order.
+        constexpr int kRowBytes = D * BITS / 8;
+        const int mix = kSub == 1 ? 0 : (kRowBytes >= 128 ? key0 : key0 >> 1) & 1;
         uint32_t chunk[kChunks];
 #pragma unroll
         for (int i = 0; i < kChunks; ++i) chunk[i] = key0 * 128 + (((kChunks * piece + i) ^ (key0 & 7)) << 4);
         const uint32_t from = smem_at(a.l.stage) + key0 * kRowBytes + piece * 16;
         const bool halves = a.stage_rows < kKeys;
-        // Scales: a warp unpacks the same 16 keys of every tile, so it keeps their tables for itself; when it comes to a
-        // tile's K its lower lanes take the 16 keys of K, the upper ones those of V, whose factor the softmax needs
-        // before V is unpacked.
-        const int lane = threadIdx.x & 31, kk = lane & 15;
-        const bool does_v = lane >= 16;
+        // Scales: a warp unpacks the same 16 keys of every tile, so it keeps their tables for itself, two lanes a key.
+        // V's are made a tile ahead of its unpacking, since the softmax needs V's factor.
+        const int lane = threadIdx.x & 31, kk = lane & 15, first = groups == 8 ? 2 * (lane >> 4) : lane >> 4;
         const int key_of = (pt >> 5) * (BITS == 8 ? 8 : 16) + (BITS == 8 ? (kk & 7) + 64 * (kk >> 3) : kk);
-        const uint32_t v_bytes = kKeys * groups * 4, tk = smem_at(kTables), tv = tk + v_bytes;
+        const uint32_t table_bytes = kKeys * groups * 4, tables = smem_at(kTables) + (is_v ? table_bytes : 0);
         Groups g;
-        Ring ring{0, 0};
-        int slot = 0;
+        Ring ring = ring_of(a, is_v);
+        const int first_slot = is_v ? a.stages : 0;
+        int slot = first_slot;
         uint32_t phase = 0;
         // look: first row of the tile to look at for non-finite values, kKeys for none
         const auto emit = [&](uint32_t table, int look, int unit) {
-            uint32_t codes[kPieces];  // kPieces x (256 / kRowThreads) rows: one slot, or two halves
+            uint32_t codes[kPieces];  // kPieces x (kGroup / kRowThreads) rows: one slot, or two halves
+            int staged[kPieces];
 #pragma unroll
             for (int x = 0; x < kPieces; ++x) {
                 if (x == 0 || halves) {
+                    staged[x] = slot;
                     codes[x] = from + slot * slot_bytes;
                     wait(&fixed().staged[slot], phase);
-                    if (++slot == a.stages) {
-                        slot = 0;
+                    if (++slot == first_slot + a.stages) {
+                        slot = first_slot;
                         phase ^= 1;
                     }
                 } else {
-                    codes[x] = codes[0] + x * (256 / kRowThreads) * kRowBytes;
+                    codes[x] = codes[0] + x * (kGroup / kRowThreads) * kRowBytes;
                 }
             }
             const uint32_t entry = table + key0 * groups * 4;
 #pragma unroll
-            for (int b0 = 0; b0 < NB; b0 += kMix) {
-                int at[kMix / kSub];
+            for (int m = 0; m < MB; ++m) {
+                wait(&fixed().empty[ring.slot], ring.phase ^ 1);
+                const uint32_t box0 = ring_at + ring.slot * kSlot;
 #pragma unroll
-                for (int b = 0; b < kMix / kSub; ++b) {
-                    at[b] = ring.slot;
-                    wait(&fixed().empty[ring.slot], ring.phase ^ 1);
-                    ring.step(a.slots);
-                }
-#pragma unroll
-                for (int b = 0; b < kMix; ++b) {
-                    const int mine = b ^ mix, box = b0 + mine;  // the box this thread's row takes now
-                    uint32_t row = at[0];
-                    if (kMix / kSub > 1) row = mine / kSub ? at[kMix / kSub - 1] : at[0];
-                    row = ring_at + row * kSlot + (mine % kSub) * kBox;
+                for (int b = 0; b < kSub; ++b) {
+                    const int mine = b ^ mix, box = m * kSub + mine;  // the box this thread's row takes now
                     const uint32_t sb = entry + ((box * 64 + piece * (128 / BITS)) >> shift) * 4;
 #pragma unroll
                     for (int x = 0; x < kPieces; ++x)
-                        unpack(lds128(codes[x] + box * (8 * BITS)), lds32(sb + x * (256 / kRowThreads) * groups * 4),
-                               row + x * (256 / kRowThreads) * 128, chunk);
+                        unpack(lds128(codes[x] + box * (8 * BITS)), lds32(sb + x * (kGroup / kRowThreads) * groups * 4),
+                               box0 + mine * kBox + x * (kGroup / kRowThreads) * 128, chunk);
                 }
                 if (__builtin_expect(look < kKeys, 0))
-#pragma unroll
-                    for (int b = 0; b < kMix; ++b)
-                        take_out(ring_at + at[b / kSub] * kSlot + (b % kSub) * kBox, look, pt,
-                                 &fixed().poison[unit & (kPoison - 1)]);
-                __syncwarp();
-                if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-                    for (int b = 0; b < kMix / kSub; ++b) mbar_arrive(&fixed().full[at[b]]);
-                }
+#pragma unroll 1
+                    for (int b = 0; b < kSub; ++b) take_out(box0 + b * kBox, look, pt, &fixed().poison[unit & (kPoison - 1)]);
+                signal_full(ring.slot);
+                ring.step();
             }
             if ((threadIdx.x & 31) == 0) {  // the codes have been read
-                const int last = slot == 0 ? a.stages - 1 : slot - 1;
-                mbar_arrive(&fixed().unstaged[last]);
-                if (halves) mbar_arrive(&fixed().unstaged[last == 0 ? a.stages - 1 : last - 1]);
+#pragma unroll
+                for (int x = 0; x < kPieces; ++x)
+                    if (x == 0 || halves) mbar_arrive(&fixed().unstaged[staged[x]]);
             }
         };
         Unit u;
         if (!w.next(a, u)) return;
         Source cur(a, u), next;
-        load_groups(a, cur, does_v, cur.t0 * kKeys + key_of, groups, g);
+        load_groups(a, cur, is_v, cur.t0 * kKeys + key_of, groups, first, g);
         int tile = 0;
-        bool more = true;
+        bool more = true, bad = false;
         for (int unit = 0; more; ++unit) {
             more = w.next(a, u);
             if (more) next = Source(a, u);
 #pragma unroll 1
-            for (int i = 0; i <= cur.n; ++i, ++tile) {
+            for (int i = 0; i <= cur.n; ++i, ++tile) {  // K(i), V(i - 1)
+                const bool bad_before = bad;
                 if (i < cur.n) {
                     const int depth = tile % kScaleDepth;
                     wait(&fixed().sc_empty[depth], ((tile / kScaleDepth) & 1) ^ 1);
-                    const float top = largest(g, groups);
-                    if (does_v) {
-                        const int e = min(max(exponent(top), -15), 24);
-                        store_groups(tv + (tile & 1) * v_bytes + key_of * groups * 4, g, groups, exp2i(kTop - e));
-                        fixed().key_v[depth][key_of] = e;
-                        fixed().key_w[depth][key_of] = static_cast<uint16_t>(pack2<false>(exp2i(-e), 0.f));
-                    } else {
-                        const int e = min(max(exponent(top), -100), 120);
-                        store_groups(tk + key_of * groups * 4, g, groups, exp2i(kTop - e));
-                        fixed().key_k[depth][key_of] = exp2i(e - kTop);
+                    float top = largest(g);
+                    const float other = __shfl_xor_sync(0xffffffffu, top, 16);
+                    asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(other));
+                    const int e = min(max(exponent(top), -100), 100);
+                    store_groups(tables + (is_v ? (tile & 1) * table_bytes : 0) + key_of * groups * 4, g, groups, first,
+                                 exp2i(kTop - e));
+                    if (lane < 16) {
+                        if (is_v) {
+                            fixed().key_v[depth][key_of] = e;
+                        } else {
+                            fixed().key_k[depth][key_of] = exp2i(e - kTop);
+                        }
                     }
-                    __syncwarp();
+                    bad = __any_sync(0xffffffffu, !(top < INFINITY));
                     if (lane == 0) mbar_arrive(&fixed().sc_full[depth]);
-                    if (i + 1 < cur.n) load_groups(a, cur, does_v, (cur.t0 + i + 1) * kKeys + key_of, groups, g);
-                    else if (more) load_groups(a, next, does_v, next.t0 * kKeys + key_of, groups, g);
-                    emit(tk, kKeys, 0);
+                    if (i + 1 < cur.n) load_groups(a, cur, is_v, (cur.t0 + i + 1) * kKeys + key_of, groups, first, g);
+                    else if (more) load_groups(a, next, is_v, next.t0 * kKeys + key_of, groups, first, g);
+                    if (!is_v) emit(tables, kKeys, 0);
                 }
-                if (i > 0) {
+                if (is_v && i > 0) {
                     const int at = (cur.t0 + i - 1) * kKeys, look = max(0, cur.hidden - at);
-                    emit(tv + ((tile - 1) & 1) * v_bytes, at + look < cur.keys ? look : kKeys, unit);
+                    emit(tables + ((tile - 1) & 1) * table_bytes, bad_before && at + look < cur.keys ? look : kKeys, unit);
                 }
             }
             --tile;  // the unit's last pass was V alone
@@ -657,7 +647,8 @@ struct Kernel {
     __device__ static void issue(const Args& a, uint32_t tmem_lane) {
         const bool one = tc5::elect();
         const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_lane, 0);
-        Ring ring{0, 0};
+        Ring rk = ring_of(a, false), rv_own = ring_of(a, true);
+        Ring& rv = kQuant ? rv_own : rk;
         int tile = 0;
         const uint32_t q = smem_at(a.l.q), p = smem_at(a.l.p);
 #pragma unroll 1
@@ -673,9 +664,9 @@ struct Kernel {
                 const uint32_t d = tmem + ((tile + i) & 1) * a.nr;
 #pragma unroll 1
                 for (int b = 0; b < MB; ++b) {
-                    wait(&fixed().full[ring.slot], ring.phase);
+                    wait(&fixed().full[rk.slot], rk.phase);
                     fence_proxy_async_shared();
-                    const uint32_t k = smem_at(a.l.ring) + ring.slot * kSlot, qb = q + b * kSub * a.nr * 128;
+                    const uint32_t k = smem_at(a.l.ring) + rk.slot * kSlot, qb = q + b * kSub * a.nr * 128;
                     const uint64_t dk = tc5::operand(k, 16, 1024), dq = tc5::operand(qb, 16, 1024);
                     const uint32_t q_step = a.nr * 128 / 16;
                     if (one) {
@@ -684,9 +675,9 @@ struct Kernel {
 #pragma unroll
                             for (int ks = 0; ks < 4; ++ks)  // 32 bytes on
                                 tc5::mma(d, dk + y * (kBox / 16) + ks * 2, dq + y * q_step + ks * 2, desc_qk, b + y + ks > 0);
-                        tc5::commit(&fixed().empty[ring.slot]);
+                        tc5::commit(&fixed().empty[rk.slot]);
                     }
-                    ring.step(a.slots);
+                    rk.step();
                 }
                 if (one) tc5::commit(&fixed().s_full[(tile + i) & 1]);
             };
@@ -698,9 +689,9 @@ struct Kernel {
                 tc5::fence_after();
 #pragma unroll 1
                 for (int mb = 0; mb < MB; ++mb) {
-                    const int slot = ring.slot;
-                    wait(&fixed().full[slot], ring.phase);
-                    ring.step(a.slots);
+                    const int slot = rv.slot;
+                    wait(&fixed().full[slot], rv.phase);
+                    rv.step();
                     fence_proxy_async_shared();
                     const uint64_t dv = tc5::operand(smem_at(a.l.ring) + slot * kSlot, kBox, 1024);
                     const uint64_t dp = tc5::operand(p, kBox, 1024);
@@ -724,7 +715,7 @@ struct Kernel {
     __device__ static __forceinline__ void load_q(const Args& a, const Unit& u) {
         constexpr int kPer = D / 8, kBatch = 4;  // 16-byte pieces of a row, which sit in one warp; loads in flight
         const int tid = threadIdx.x;
-        const int t0 = u.block * kRows / a.G, g0 = u.block * kRows - t0 * a.G;
+        const int t0 = u.block * a.rb / a.G, g0 = u.block * a.rb - t0 * a.G;
         const uint16_t* base = a.q + ((u.prefix ? 0 : (int64_t)u.seq * a.tokens) + t0) * a.ld_q + (size_t)u.head * a.G * D;
         // row n of the block is token t0 + v / G, head v % G of v = g0 + n < 256: a product with 2^16 / G
         const auto token_of = [&](int n) { return static_cast<int>(static_cast<uint32_t>((g0 + n) * a.g_magic) >> 16); };
@@ -785,8 +776,6 @@ struct Kernel {
         const int key = quarter * 32 + lane, tid = threadIdx.x & 127;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const int columns = a.nr / 2, c0 = half * columns;  // this warp's columns of S^T
-        const int l_cols = a.nr / 8, l0 = warp * l_cols;    // columns whose sums it forms (inside its half)
-        constexpr uint32_t ones = 0x3f803f80u;
         const float qscale = a.scale * 1.4426950408889634f;
         int tile = 0, units = 0;
         Unit u;
@@ -800,7 +789,7 @@ struct Kernel {
                 fixed().unit_rows = u.rows;
                 mbar_arrive(&fixed().q_full);
             }
-            float lsum[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            float l0 = 0.f, l1 = 0.f;  // sums over this warp's keys: lane j has column c0 + j, and c0 + 32 + j
             for (int i = 0; i < u.n; ++i, ++tile) {
                 const int depth = tile % kScaleDepth;
                 float ks = 1.f, ev = 0.f;
@@ -815,8 +804,16 @@ struct Kernel {
                 const int b = at + key - u.len;  // block row of the key; a prefix ends where its block would begin
                 const bool masked = at + kKeys > u.len;
                 bool waited = i == 0;  // for the last tile's p V: P and the accumulators are free
+                const int end = min(c0 + columns, u.rows);
+                const float weight = kQuant ? exp2i(-static_cast<int>(ev)) : 1.f;
+                const auto hand_over = [&]() {
+                    fence_proxy_async_shared();
+                    tc5::fence_before();
+                    named_bar_sync(1 + half, 128);
+                    if (tid == 0) mbar_arrive(&fixed().p_full);
+                };
 #pragma unroll 1
-                for (int n0 = c0; n0 < min(c0 + columns, u.rows); n0 += 32) {  // 32 columns at a time in registers
+                for (int n0 = c0; n0 < end; n0 += 32) {  // 32 columns at a time in registers
                     float y[32];
                     tc5::ld32(tmem + lanes + (tile & 1) * a.nr + n0, y);
                     if (kQuant) {
@@ -891,62 +888,33 @@ struct Kernel {
                                 }
                             tc5::wait_st();
                         }
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {  // and the sums, each warp its own columns
-                            const int n = l0 + 8 * x + 2 * (lane & 3);
-                            if (8 * x < l_cols && n >= n0 && n < n0 + 32) {
-                                if (n < u.rows) lsum[x][0] *= fixed().corr[n];
-                                if (n + 1 < u.rows) lsum[x][1] *= fixed().corr[n + 1];
-                            }
-                        }
+                        if (n0 + lane < u.rows) (n0 == c0 ? l0 : l1) *= fixed().corr[n0 + lane];  // and the sums
                     }
                     const uint32_t row = smem_at(a.l.p) + (n0 >> 6) * kBox + key * 128;
 #pragma unroll
                     for (int j = 0; j < 32; j += 8) {
                         const float4 ma = *reinterpret_cast<const float4*>(&fixed().mm[n0 + j]);
                         const float4 mb = *reinterpret_cast<const float4*>(&fixed().mm[n0 + j + 4]);
-                        uint4 v;
-                        v.x = pack2<!kQuant>(ex2(y[j] - ma.x), ex2(y[j + 1] - ma.y));
-                        v.y = pack2<!kQuant>(ex2(y[j + 2] - ma.z), ex2(y[j + 3] - ma.w));
-                        v.z = pack2<!kQuant>(ex2(y[j + 4] - mb.x), ex2(y[j + 5] - mb.y));
-                        v.w = pack2<!kQuant>(ex2(y[j + 6] - mb.z), ex2(y[j + 7] - mb.w));
-                        sts128(row + (((((n0 & 63) + j) >> 3) ^ (key & 7)) << 4), v);
-                    }
-                }
-                if (!waited) {  // no columns of its own
-                    wait(&fixed().pv_done, (tile - 1) & 1);
-                    tc5::fence_after();
-                }
-                fence_proxy_async_shared();
-                tc5::fence_before();
-                named_bar_sync(1 + half, 128);
-                if (tid == 0) mbar_arrive(&fixed().p_full);
-                // sums of the columns over the tile's keys: one 16-row product with a row of ones (or of
-                // the keys' weights), on the rounded P that the numerator uses
+                        const float m8[8] = {ma.x, ma.y, ma.z, ma.w, mb.x, mb.y, mb.z, mb.w};
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int n = l0 + 8 * x;
-                    if (8 * x < l_cols && n < u.rows) {
-                        const uint32_t box = smem_at(a.l.p) + (n >> 6) * kBox;
-#pragma unroll
-                        for (int kk = 0; kk < kKeys; kk += 32) {
-                            const int r = kk + lane;
-                            uint32_t b0, b1, b2, b3;
-                            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                                         : "=r"(b0), "=r"(b1), "=r"(b2), "=r"(b3)
-                                         : "r"(box + r * 128 + (((((n & 63) >> 3)) ^ (r & 7)) << 4))
-                                         : "memory");
-                            if constexpr (kQuant) {
-                                const uint32_t kw = smem_u32(&fixed().key_w[depth][kk + 2 * (lane & 3)]);
-                                const uint32_t a0 = lds32(kw), a2 = lds32(kw + 16), a4 = lds32(kw + 32), a6 = lds32(kw + 48);
-                                mma_f16_16816(lsum[x], a0, a0, a2, a2, b0, b1);
-                                mma_f16_16816(lsum[x], a4, a4, a6, a6, b2, b3);
-                            } else {
-                                mma_bf16_16816(lsum[x], ones, ones, ones, ones, b0, b1);
-                                mma_bf16_16816(lsum[x], ones, ones, ones, ones, b2, b3);
-                            }
-                        }
+                        for (int x = 0; x < 8; ++x) y[j + x] = ex2(y[j + x] - m8[x]);
+                        sts128(row + (((((n0 & 63) + j) >> 3) ^ (key & 7)) << 4),
+                               make_uint4(pack2<!kQuant>(y[j], y[j + 1]), pack2<!kQuant>(y[j + 2], y[j + 3]),
+                                          pack2<!kQuant>(y[j + 4], y[j + 5]), pack2<!kQuant>(y[j + 6], y[j + 7])));
                     }
+                    if (n0 + 32 >= end) hand_over();  // before the sums, which nobody waits for
+                    if (kQuant) {  // V's factor is part of P
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) y[j] *= weight;
+                    }
+                    (n0 == c0 ? l0 : l1) += stack::reduce_scatter32(y, lane);
+                }
+                if (c0 >= end) {  // no columns of its own
+                    if (i > 0) {
+                        wait(&fixed().pv_done, (tile - 1) & 1);
+                        tc5::fence_after();
+                    }
+                    hand_over();
                 }
                 if (kQuant) {
                     __syncwarp();
@@ -970,14 +938,13 @@ struct Kernel {
                     }
                 }
             }
-            if (lane < 4) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    if (8 * x < l_cols) {
-                        const int n = l0 + 8 * x + 2 * lane;
-                        if (n < u.rows) a.ml[at + n] = make_float2(fixed().m[n], lsum[x][0]);
-                        if (n + 1 < u.rows) a.ml[at + n + 1] = make_float2(fixed().m[n + 1], lsum[x][1]);
-                    }
+            if (c0 + lane < u.rows) fixed().part[quarter][c0 + lane] = l0;
+            if (columns > 32 && c0 + 32 + lane < u.rows) fixed().part[quarter][c0 + 32 + lane] = l1;
+            named_bar_sync(1 + half, 128);
+            if (tid < columns && c0 + tid < u.rows) {
+                const int n = c0 + tid;
+                a.ml[at + n] = make_float2(fixed().m[n], (fixed().part[0][n] + fixed().part[1][n]) +
+                                                             (fixed().part[2][n] + fixed().part[3][n]));
             }
             if (threadIdx.x == 0) {
                 const long long seg = (u.prefix ? 0 : segments_p(a)) + u.segment;
@@ -1057,7 +1024,7 @@ struct Kernel {
         const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
         if (threadIdx.x == 0) {
             for (int i = 0; i < kMaxSlots; ++i) {
-                mbar_init(&fixed().full[i], kQuant ? kProducerWarps : 32 * kProducerWarps);
+                mbar_init(&fixed().full[i], kQuant ? kProducerWarps : kGroup);
                 mbar_init(&fixed().empty[i], 1);
             }
             mbar_init(&fixed().s_full[0], 1);
@@ -1066,7 +1033,7 @@ struct Kernel {
             mbar_init(&fixed().pv_done, 1);
             mbar_init(&fixed().q_full, 1);
             for (int i = 0; i < kScaleDepth; ++i) {
-                mbar_init(&fixed().sc_full[i], kProducerWarps);
+                mbar_init(&fixed().sc_full[i], 2 * kProducerWarps);
                 mbar_init(&fixed().sc_empty[i], kSoftmaxWarps);
             }
             for (int i = 0; i < kMaxStages; ++i) {
@@ -1077,7 +1044,7 @@ struct Kernel {
             fence_barrier_init();
         }
         if (threadIdx.x < kPoison) fixed().poison[threadIdx.x] = 0;
-        if (warp == kSoftmaxWarps + kProducerWarps) tc5::alloc(smem_u32(&fixed().tmem), kTmemColumns);
+        if (warp == kIssueWarp) tc5::alloc(smem_u32(&fixed().tmem), kTmemColumns);
         pdl_wait();
         pdl_launch_dependents();
         plan(a);
@@ -1089,19 +1056,19 @@ struct Kernel {
         if (warp < kSoftmaxWarps) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             softmax(a, w, tmem, blockIdx.x);
-        } else if (warp < kSoftmaxWarps + kProducerWarps) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
-            if constexpr (kQuant) produce_quant(a, w);
+        } else if (warp < kIssueWarp) {
+            if constexpr (kQuant) produce_quant(a, w, warp >= kSoftmaxWarps + kProducerWarps);
             else produce_bf16(a, w);
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-            if (warp == kSoftmaxWarps + kProducerWarps) issue(a, tmem);
-            else if (kQuant && threadIdx.x == 32 * (kSoftmaxWarps + kProducerWarps + 1)) stage(a, w);
+            if (warp == kIssueWarp) issue(a, tmem);
+            else if (kQuant && (warp == kIssueWarp + 1 || warp == kIssueWarp + 2) && (threadIdx.x & 31) == 0)
+                stage(a, w, warp == kIssueWarp + 2);
             __syncwarp();
         }
         tc5::fence_before();
         __syncthreads();
-        if (warp == kSoftmaxWarps + kProducerWarps) tc5::dealloc(tmem, kTmemColumns);
+        if (warp == kIssueWarp) tc5::dealloc(tmem, kTmemColumns);
     }
 };
 
@@ -1138,7 +1105,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
         const bool prefix = side == 0;
         if (prefix && a.blocks_p == 0) continue;
         const long long row = prefix ? (long long)r * a.G + g : (long long)t * a.G + g;
-        const int block = static_cast<int>(row / kRows), n = static_cast<int>(row % kRows);
+        const int block = static_cast<int>(row / a.rb), n = static_cast<int>(row % a.rb);
         const long long seg = prefix ? (long long)block * a.cache.hkv + head
                                      : ((long long)seq * a.blocks_o + block) * a.cache.hkv + head;
         const long long meta = (prefix ? 0 : segments_p(a)) + seg;
@@ -1214,15 +1181,19 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     kv::store_lane<CH>(out, acc);
 }
 
+// Query rows of a block: kRows, but 64 over quantised caches of 256 dims, where Q and P of 128 rows would leave the codes no
+// room in shared memory.
+static int row_block(const dflash_kv_cache& c) { return c.bits != 16 && c.head_dim == 256 ? 64 : kRows; }
+
 static int check(const dflash_kv_cache* cache, const dflash_kv_cache* prefix, int prefix_len, int tokens, int hq,
                  const char* who) {
     const int st = kv::check_cache(cache, who);
     if (st != DFLASH_OK) return st;
     if (tokens < 1 || tokens > cache->max_len || hq < 1 || hq % cache->kv_heads || prefix_len < 0)
         return fail(DFLASH_ERR_INVALID_ARGUMENT, "%s: bad arguments", who);
-    const long long G = hq / cache->kv_heads, tiles = (cache->max_len + kKeys - 1ll) / kKeys;
-    const long long blocks_p = prefix_len ? ((long long)cache->sequences * tokens * G + kRows - 1) / kRows : 0;
-    const long long blocks_o = ((long long)tokens * G + kRows - 1) / kRows;
+    const long long G = hq / cache->kv_heads, rb = row_block(*cache), tiles = (cache->max_len + kKeys - 1ll) / kKeys;
+    const long long blocks_p = prefix_len ? ((long long)cache->sequences * tokens * G + rb - 1) / rb : 0;
+    const long long blocks_o = ((long long)tokens * G + rb - 1) / rb;
     if (G > 64 || (long long)cache->sequences * tokens > 0x7fffffffll / hq ||
         (long long)prefix_len + cache->max_len > 0x7fffffffll - kKeys ||
         blocks_p * cache->kv_heads * ((prefix_len + kKeys - 1ll) / kKeys) +
@@ -1248,25 +1219,37 @@ static size_t fit(Args& a, const dflash_kv_cache& c, int prefix_len, int tokens,
     a.hq = hq;
     a.G = hq / c.kv_heads;
     a.g_magic = (65536 + a.G - 1) / a.G;  // v / G exactly for v < 256, G <= 64: v (G - 1) < 2^16
+    a.rb = row_block(c);
     const long long rows_p = (long long)c.sequences * tokens * a.G, rows_o = (long long)tokens * a.G;
-    a.blocks_p = prefix_len ? static_cast<int>((rows_p + kRows - 1) / kRows) : 0;
-    a.blocks_o = static_cast<int>((rows_o + kRows - 1) / kRows);
-    a.rows_o = static_cast<int>(rows_o < kRows ? rows_o : kRows);
-    a.nr = (prefix_len ? rows_p : rows_o) <= 64 ? 64 : kRows;
+    a.blocks_p = prefix_len ? static_cast<int>((rows_p + a.rb - 1) / a.rb) : 0;
+    a.blocks_o = static_cast<int>((rows_o + a.rb - 1) / a.rb);
+    a.rows_o = static_cast<int>(rows_o < a.rb ? rows_o : a.rb);
+    a.nr = a.rb == 64 || (prefix_len ? rows_p : rows_o) <= 64 ? 64 : kRows;
     const int groups = c.bits == 16 ? 0 : c.head_dim / c.group;
-    // bf16: all that fits in ring slots.  Quantised: ring slots for a K or V tile and a half, then staging slots of
-    // whole tiles; of half tiles where two whole ones do not fit, and then fewer ring slots.
-    const int quant = c.bits != 16, sub = c.head_dim > 64 ? 2 : 1, row_bytes = c.head_dim * c.bits / 8;
-    a.stage_rows = kKeys;
-    const auto fits = [&](int slots, int stages) {
-        return layout(c.head_dim, a.nr, slots, stages, a.stage_rows * row_bytes, groups).total <= kSmemLimit;
+    // bf16: all that fits in ring slots.  Quantised: as many slots of two for K and two for V as leave each two
+    // staging slots, of whole tiles or (8 bits) of halves.
+    const int sub = c.head_dim > 64 ? 2 : 1, row_bytes = c.head_dim * c.bits / 8;
+    const auto fits = [&](int slots, int stages, int rows) {
+        return layout(c.head_dim, a.nr, slots, stages, rows * row_bytes, groups).total <= kSmemLimit;
     };
-    a.stages = quant ? 2 : 0;
-    a.slots = quant ? (c.head_dim == 256 ? 3 : 4) : kMaxSlots / sub;
-    if (c.bits == 8 && !fits(a.slots, 2)) a.stage_rows = kKeys / 2;
-    while (!fits(a.slots, a.stages)) --a.slots;
-    while (quant && a.stages < kMaxStages && fits(a.slots, a.stages + 1)) ++a.stages;
-    a.l = layout(c.head_dim, a.nr, a.slots, a.stages, a.stage_rows * row_bytes, groups);
+    a.stages = 0;
+    a.stage_rows = kKeys;
+    if (c.bits == 16) {
+        a.slots = kMaxSlots / sub;
+        while (!fits(a.slots, 0, 0)) --a.slots;
+        a.slots_k = a.slots;
+    } else {
+        for (a.slots = 4; a.slots >= 2 && a.stages == 0; --a.slots)
+            for (int rows = kKeys; rows >= (c.bits == 8 ? kKeys / 2 : kKeys) && a.stages == 0; rows /= 2)
+                for (int n = kMaxStages / 2; n >= 2 && a.stages == 0; --n)
+                    if (fits(a.slots, 2 * n, rows)) {
+                        a.stages = n;
+                        a.stage_rows = rows;
+                    }
+        ++a.slots;
+        a.slots_k = (a.slots + 1) / 2;
+    }
+    a.l = layout(c.head_dim, a.nr, a.slots, 2 * a.stages, a.stage_rows * row_bytes, groups);
     size_t at = 0;
     const auto take = [&](size_t bytes) {
         uint8_t* p = base + at;
@@ -1274,7 +1257,7 @@ static size_t fit(Args& a, const dflash_kv_cache& c, int prefix_len, int tokens,
         return p;
     };
     const size_t segs = segments_p(a) + segments_o(a), parts = partials_p(a) + partials_o(a);
-    const size_t rows = partials_p(a) * kRows + partials_o(a) * a.rows_o;
+    const size_t rows = partials_p(a) * a.rb + partials_o(a) * a.rows_o;
     a.first = reinterpret_cast<int32_t*>(take(4 * segs));
     a.last = reinterpret_cast<int32_t*>(take(4 * segs));
     a.poison = reinterpret_cast<int32_t*>(take(4 * parts));

@@ -365,6 +365,26 @@ def test_attention_is_the_same_every_time(dc, cuda):
         assert torch.equal(f(), first)
 
 
+@pytest.mark.parametrize("case", [
+    (2, 509, 16, 2, 128, 8, 32, [7000, 3100], 0), (1, 8, 24, 4, 256, 8, 64, [20000], 0), (3, 2, 24, 4, 256, 4, 32, [9000, 4000, 1], 700),
+    (2, 40, 24, 4, 256, 8, 32, [5000, 100], 0), (4, 16, 8, 1, 64, 4, 32, [3000, 10, 8000, 400], 2000),
+    (2, 100, 8, 2, 256, 16, 0, [6000, 50], 1000), (9, 3, 16, 2, 128, 4, 128, [1000 * i for i in range(9)], 5000),
+], ids=str)
+def test_long_runs_of_tiles_back_to_back(dc, cuda, case):
+    """Many tiles per CTA, calls that follow each other without a pause, and every call the same bits:
+    what a slot reused too early or a wait for the wrong phase would change."""
+    q, gate, cache, prefix, _ = attention_case(dc, cuda, case, seed=71)
+    lens = lens_tensor(case[7], cuda)
+    f = lambda: dc.stack_attn_decode_batch(q, cache, lens, case[4] ** -0.5, gate=gate, prefix=prefix,  # noqa: E731
+                                           prefix_len=case[8])
+    outs = [f() for _ in range(40)]
+    torch.cuda.synchronize()
+    assert dc.device_error() == 0
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    want, tol = attention_want(q, gate, cache, prefix, None, case, case[4] ** -0.5)
+    check_rows(outs[0], want, tol)
+
+
 def test_an_offset_past_32_bits(dc, cuda):
     """The last rows of a cache of 5 GB: element offsets pass 2^32."""
     hkv, d, max_len = 2, 256, 4_200_000
