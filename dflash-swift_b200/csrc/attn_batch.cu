@@ -49,6 +49,7 @@ constexpr int kScaleDepth = 2;             // tiles whose key factors may be ali
 constexpr int kPoison = 16;                // units whose poison flags may be alive at once
 constexpr float kLazy = 4.f;               // a maximum moves when a score passes it by 2^4 ...
 constexpr float kLift = 8.f;               // ... and P is 2^8 p, up to 2^12: small weights stay normal in fp16
+constexpr float kNever = 1e30f;            // base of a row without a maximum yet: every score passes it
 constexpr int kTopQ = 12;                  // query rows are scaled to 2^12 .. 2^13 in fp16
 constexpr uint32_t kTmemColumns = 512;
 constexpr int kSmemLimit = 232448;
@@ -58,8 +59,8 @@ constexpr int kSmemLimit = 232448;
 struct Fixed {
     uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full, pv_done, q_full, sc_full[kScaleDepth],
         sc_empty[kScaleDepth], staged[kMaxStages], unstaged[kMaxStages];
-    alignas(16) float thr[kRows];       // read four at a time, like mm and qs
-    float mm[kRows], qs[kRows], corr[kRows], m[kRows];
+    alignas(16) float base[kRows];      // -(maximum - kLift): scores are taken relative to it; read four at a time, like qs
+    float qs[kRows], corr[kRows], m[kRows];
     int info[kRows];                    // chain: the row's token; tree: its path mask
     float part[4][kRows];
     float key_k[kScaleDepth][kKeys], key_v[kScaleDepth][kKeys];
@@ -68,7 +69,7 @@ struct Fixed {
     int unit_tiles, unit_rows;          // for the issuing thread, from the softmax warps
     int warp_sum[kThreads / 32];
 };
-static_assert(offsetof(Fixed, thr) % 16 == 0 && offsetof(Fixed, mm) % 16 == 0 && offsetof(Fixed, qs) % 16 == 0 &&
+static_assert(offsetof(Fixed, base) % 16 == 0 && offsetof(Fixed, qs) % 16 == 0 &&
                   alignof(Fixed) == 16, "vector accesses");
 constexpr uint32_t kTables = (sizeof(Fixed) + 15) / 16 * 16;
 
@@ -200,6 +201,20 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Two 32-bit operations in one instruction: a *= b, a += b, a = a * b + c.
+__device__ __forceinline__ void mul2(float& a0, float& a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+        "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+        "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void fma2(float& a0, float& a1, float b0, float b1, float c0, float c1) {
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\t"
+        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ float warp_max(float x) {  // NaN counts as nothing
     float y;
@@ -758,8 +773,7 @@ struct Kernel {
         if (tid < kRows) {
             const int n = tid;
             const bool live = n < u.rows;
-            fixed().thr[n] = live ? -INFINITY : INFINITY;  // a row that is not there never raises its maximum
-            fixed().mm[n] = -kLift;
+            fixed().base[n] = live ? kNever : -INFINITY;  // nothing passes that of a row that is not there
             fixed().m[n] = -INFINITY;
             // key b of the block (below 0: cached rows) is seen if b <= info, in a tree if bit b of info is set
             int info = -1;
@@ -815,46 +829,53 @@ struct Kernel {
 #pragma unroll 1
                 for (int n0 = c0; n0 < end; n0 += 32) {  // 32 columns at a time in registers
                     float y[32];
-                    tc5::ld32(tmem + lanes + (tile & 1) * a.nr + n0, y);
-                    if (kQuant) {
+                    bool raise = false;  // this pass: plain scores for new maxima, not scores relative to the old ones
+#pragma unroll 1
+                    for (int pass = 0;; ++pass) {  // one, or three with a raise: scores, plain scores, scores
+                        tc5::ld32(tmem + lanes + (tile & 1) * a.nr + n0, y);
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
-                            const float4 qs = *reinterpret_cast<const float4*>(&fixed().qs[n0 + j]);
-                            y[j] = fmaf(y[j] * ks, qs.x, ev);
-                            y[j + 1] = fmaf(y[j + 1] * ks, qs.y, ev);
-                            y[j + 2] = fmaf(y[j + 2] * ks, qs.z, ev);
-                            y[j + 3] = fmaf(y[j + 3] * ks, qs.w, ev);
+                            float4 bs = *reinterpret_cast<const float4*>(&fixed().base[n0 + j]);
+                            if (raise) bs = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (kQuant) {
+                                const float4 qs = *reinterpret_cast<const float4*>(&fixed().qs[n0 + j]);
+                                add2(bs.x, bs.y, ev, ev);
+                                add2(bs.z, bs.w, ev, ev);
+                                mul2(y[j], y[j + 1], ks, ks);
+                                mul2(y[j + 2], y[j + 3], ks, ks);
+                                fma2(y[j], y[j + 1], qs.x, qs.y, bs.x, bs.y);
+                                fma2(y[j + 2], y[j + 3], qs.z, qs.w, bs.z, bs.w);
+                            } else {
+                                fma2(y[j], y[j + 1], qscale, qscale, bs.x, bs.y);
+                                fma2(y[j + 2], y[j + 3], qscale, qscale, bs.z, bs.w);
+                            }
                         }
-                    } else {
+                        if (masked) {  // by the row's token, or its path's bits (load_q)
+                            if (a.parents && !u.prefix) {
+                                const int bit = b < 0 ? -1 : b < 32 ? 1 << b : 0;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) y[j] *= qscale;
-                    }
-                    if (masked) {  // by the row's token, or its path's bits (load_q)
-                        if (a.parents && !u.prefix) {
-                            const int bit = b < 0 ? -1 : b < 32 ? 1 << b : 0;
+                                for (int j = 0; j < 32; ++j) y[j] = fixed().info[n0 + j] & bit ? y[j] : -INFINITY;
+                            } else {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) y[j] = fixed().info[n0 + j] & bit ? y[j] : -INFINITY;
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) y[j] = b <= fixed().info[n0 + j] ? y[j] : -INFINITY;
+                                for (int j = 0; j < 32; ++j) y[j] = b <= fixed().info[n0 + j] ? y[j] : -INFINITY;
+                            }
                         }
-                    }
-                    bool over[4] = {false, false, false, false};
+                        if (!raise) {
+                            float top[4] = {y[0], y[1], y[2], y[3]};  // NaN counts as nothing
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 th = *reinterpret_cast<const float4*>(&fixed().thr[n0 + j]);
-                        over[0] |= y[j] > th.x;
-                        over[1] |= y[j + 1] > th.y;
-                        over[2] |= y[j + 2] > th.z;
-                        over[3] |= y[j + 3] > th.w;
-                    }
-                    const bool raise = bar_any(1 + half, 128, (over[0] | over[1]) | (over[2] | over[3]));
-                    if (!waited) {
-                        wait(&fixed().pv_done, (tile - 1) & 1);
-                        tc5::fence_after();
-                        waited = true;
-                    }
-                    if (raise) {
+                            for (int j = 4; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], y[j]);
+                            if (pass == 0)
+                                raise = bar_any(1 + half, 128,
+                                                fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kLazy + kLift);
+                            if (!waited) {
+                                wait(&fixed().pv_done, (tile - 1) & 1);
+                                tc5::fence_after();
+                                waited = true;
+                            }
+                            if (!raise) break;
+                            continue;
+                        }
+                        raise = false;
                         float mine = -INFINITY;
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
@@ -870,8 +891,7 @@ struct Kernel {
                                                         fmaxf(fixed().part[2][n], fixed().part[3][n])), old);
                             fixed().corr[n] = m == old ? 1.f : ex2(old - m);
                             fixed().m[n] = m;
-                            fixed().thr[n] = m + kLazy;
-                            fixed().mm[n] = (m == -INFINITY ? 0.f : m) - kLift;
+                            if (m > -INFINITY) fixed().base[n] = kLift - m;
                         }
                         named_bar_sync(1 + half, 128);
                         if (i > 0 && (D > 64 || quarter < 2)) {  // the accumulators so far go to the new maxima
@@ -893,11 +913,8 @@ struct Kernel {
                     const uint32_t row = smem_at(a.l.p) + (n0 >> 6) * kBox + key * 128;
 #pragma unroll
                     for (int j = 0; j < 32; j += 8) {
-                        const float4 ma = *reinterpret_cast<const float4*>(&fixed().mm[n0 + j]);
-                        const float4 mb = *reinterpret_cast<const float4*>(&fixed().mm[n0 + j + 4]);
-                        const float m8[8] = {ma.x, ma.y, ma.z, ma.w, mb.x, mb.y, mb.z, mb.w};
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) y[j + x] = ex2(y[j + x] - m8[x]);
+                        for (int x = 0; x < 8; ++x) y[j + x] = ex2(y[j + x]);
                         sts128(row + (((((n0 & 63) + j) >> 3) ^ (key & 7)) << 4),
                                make_uint4(pack2<!kQuant>(y[j], y[j + 1]), pack2<!kQuant>(y[j + 2], y[j + 3]),
                                           pack2<!kQuant>(y[j + 4], y[j + 5]), pack2<!kQuant>(y[j + 6], y[j + 7])));
@@ -905,7 +922,7 @@ struct Kernel {
                     if (n0 + 32 >= end) hand_over();  // before the sums, which nobody waits for
                     if (kQuant) {  // V's factor is part of P
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) y[j] *= weight;
+                        for (int j = 0; j < 32; j += 2) mul2(y[j], y[j + 1], weight, weight);
                     }
                     (n0 == c0 ? l0 : l1) += stack::reduce_scatter32(y, lane);
                 }
@@ -1247,7 +1264,7 @@ static size_t fit(Args& a, const dflash_kv_cache& c, int prefix_len, int tokens,
                         a.stage_rows = rows;
                     }
         ++a.slots;
-        a.slots_k = (a.slots + 1) / 2;
+        a.slots_k = a.slots / 2;  // of three, two for V: its products wait for P, K's run a tile ahead
     }
     a.l = layout(c.head_dim, a.nr, a.slots, 2 * a.stages, a.stage_rows * row_bytes, groups);
     size_t at = 0;
