@@ -28,6 +28,7 @@
 #include "dflash_batch.h"
 #include "tcgen05.cuh"
 
+#include <atomic>
 #include <cstddef>
 
 namespace dflash {
@@ -1285,8 +1286,15 @@ static size_t fit(Args& a, const dflash_kv_cache& c, int prefix_len, int tokens,
 
 template <int BITS, int D>
 static cudaError_t launch(const Args& a, int ctas, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(attn_batch_kernel<BITS, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+    static std::atomic<unsigned long long> ready{0};  // devices that know the kernel's shared memory, a bit each
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    if (dev >= 64 || !((ready.load() >> dev) & 1)) {
+        e = cudaFuncSetAttribute(attn_batch_kernel<BITS, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(1ull << dev);
+    }
     e = launch_chained(attn_batch_kernel<BITS, D>, dim3(ctas), dim3(kThreads), a.l.total, s, 1, a);
     if (e != cudaSuccess) return e;
     const long long items = (long long)a.cache.sequences * a.tokens * a.hq;

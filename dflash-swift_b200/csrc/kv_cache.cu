@@ -172,42 +172,54 @@ __device__ __forceinline__ void store_cache_row(const View& cache, bool is_v, in
     }
 }
 
-// Attention prep of a batch, one warp per (row, head slot): slot < hq a q head, < hq + hkv a k
-// head, else a v head.  Lane l holds elements [l CH, l CH + CH) of the head, so every load and
-// store of a row is one coalesced access and a group of the quantisation is a run of lanes.
-// Rotary: element i < rot / 2 pairs with i + rot / 2, which a whole number of lanes further on
-// holds (rot / 2 is a multiple of 32).  The angle is kept as a fraction of a turn in 64-bit
-// fixed point: position times the frequency's fraction wraps as the angle does, so far
-// positions lose nothing (a float product is off by 2^-24 of the angle, 0.06 rad at a million).
-// The normalised k stays in 32 bits up to its one rounding, the quantisation.
-constexpr int kPrepThreads = 256;
+// Attention prep of a batch.  A CTA takes `rows_per` rows and `slots_per` head slots of each (slot < hq a q
+// head, < hq + hkv a k head, else a v head), a warp one head at a time.  Lane l holds elements
+// [l CH, l CH + CH) of the head, so every load and store of a row is one coalesced access and a group of
+// the quantisation is a run of lanes.  Rotary: element i < rot / 2 pairs with i + rot / 2, which a whole
+// number of lanes further on holds (rot / 2 is a multiple of 32); the rows' cosines and sines are made
+// once per CTA and shared by its heads.  The angle is kept as a fraction of a turn in 64-bit fixed point:
+// position times the frequency's fraction wraps as the angle does, so far positions lose nothing (a
+// float product is off by 2^-24 of the angle, 0.06 rad at a million).  The normalised k stays in 32 bits up
+// to its one rounding, the quantisation.
+constexpr int kPrepThreads = 256, kPrepRows = 8;
 
 template <int CH>
 __global__ void __launch_bounds__(kPrepThreads) attn_prep_batch_kernel(
     const uint16_t* qkv, long long ld, const uint16_t* __restrict__ q_norm, const uint16_t* __restrict__ k_norm,
     uint16_t* q_out, long long ld_q, View cache, const int32_t* __restrict__ lengths, int tokens, int hq, int rot,
-    int position0, float eps, float theta, const int32_t* __restrict__ parents) {
+    int position0, float eps, float theta, const int32_t* __restrict__ parents, int rows_per, int slots_per) {
     constexpr int d = CH * 32;
     __shared__ unsigned long long s_turn[d / 2];  // turns per position of pair i, 0.64 fixed point
-    for (int i = threadIdx.x; i < rot / 2; i += kPrepThreads) {
+    __shared__ __align__(16) float s_cos[kPrepRows][d / 2], s_sin[kPrepRows][d / 2];
+    __shared__ int s_start[kPrepRows];            // first cache row of the row's block, -1: takes no part
+    const int half = rot / 2;
+    for (int i = threadIdx.x; i < half; i += kPrepThreads) {
         const double turns = exp2(-2.0 * i / rot * log2(static_cast<double>(theta))) * 0.15915494309189533577;
         s_turn[i] = static_cast<unsigned long long>((turns - floor(turns)) * 18446744073709551616.0);
     }
-    __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, hkv = cache.hkv, slots = hq + 2 * hkv;
-    const long long items = (long long)cache.sequences * tokens * slots;
-    const long long step = (long long)gridDim.x * (kPrepThreads / 32);
-    for (long long it = (long long)blockIdx.x * (kPrepThreads / 32) + (threadIdx.x >> 5); it < items; it += step) {
-        const int r = static_cast<int>(it / slots), slot = static_cast<int>(it - (long long)r * slots);
-        const int seq = r / tokens, t = r - seq * tokens;
-        const bool is_v = slot >= hq + hkv, is_q = slot < hq;
-        const uint16_t* row = qkv + (size_t)r * ld;
-        float x[CH];
-        load_lane<CH>(row + (size_t)(is_q ? slot : hq + slot) * d + lane * CH, x);
-        const int start = block_start(lengths, seq, tokens, cache.max_len);
+    const int r0 = blockIdx.x * rows_per, rows = min(rows_per, cache.sequences * tokens - r0);
+    if (threadIdx.x < rows) s_start[threadIdx.x] = block_start(lengths, (r0 + threadIdx.x) / tokens, tokens, cache.max_len);
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * half; i += kPrepThreads) {
+        const int k = i / half, e = i - k * half, seq = (r0 + k) / tokens, t = r0 + k - seq * tokens;
+        const int depth = parents ? tree_walk(parents + (size_t)seq * tokens, t).depth : t;
+        const unsigned long long a = s_turn[e] * static_cast<unsigned long long>((long long)position0 + s_start[k] + depth);
+        sincospif(static_cast<float>(static_cast<int>(a >> 32)) * 4.656612873077392578125e-10f, &s_sin[k][e], &s_cos[k][e]);
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31, hkv = cache.hkv, pair_lanes = half / CH;
+    const int slot0 = blockIdx.y * slots_per, slots = min(slots_per, hq + 2 * hkv - slot0);
+    const bool first = lane < pair_lanes, second = lane >= pair_lanes && lane < 2 * pair_lanes;
+    const int other = first ? lane + pair_lanes : second ? lane - pair_lanes : lane;
+    for (int it = threadIdx.x >> 5; it < rows * slots; it += kPrepThreads / 32) {
+        const int k = it / slots, slot = slot0 + it - k * slots, start = s_start[k];
         if (start < 0) continue;
+        const int r = r0 + k, seq = r / tokens, t = r - seq * tokens;
+        const bool is_v = slot >= hq + hkv, is_q = slot < hq;
+        float x[CH];
+        load_lane<CH>(qkv + (size_t)r * ld + (size_t)(is_q ? slot : hq + slot) * d + lane * CH, x);
         if (!is_v) {
             float w[CH];
             load_lane<CH>((is_q ? q_norm : k_norm) + lane * CH, w);
@@ -220,29 +232,19 @@ __global__ void __launch_bounds__(kPrepThreads) attn_prep_batch_kernel(
 #pragma unroll
             for (int i = 0; i < CH; ++i) x[i] = x[i] * rs * w[i];
             if (rot > 0) {
-                const int half = rot / 2 / CH;  // lanes between a pair's two elements
-                const int depth = parents ? tree_walk(parents + (size_t)seq * tokens, t).depth : t;
-                const unsigned long long pos = static_cast<unsigned long long>((long long)position0 + start + depth);
-                const bool first = lane < half, second = lane >= half && lane < 2 * half;
-                const int other = first ? lane + half : second ? lane - half : lane;
+                const int e = (second ? lane - pair_lanes : first ? lane : 0) * CH;
 #pragma unroll
                 for (int i = 0; i < CH; ++i) {
-                    const float y = __shfl_sync(0xffffffffu, x[i], other);
-                    if (first || second) {
-                        const unsigned long long a = s_turn[(first ? lane : lane - half) * CH + i] * pos;
-                        float sn, cs;
-                        sincospif(static_cast<float>(static_cast<int>(a >> 32)) * 4.656612873077392578125e-10f, &sn, &cs);
-                        x[i] = first ? x[i] * cs - y * sn : x[i] * cs + y * sn;
-                    }
+                    const float y = __shfl_sync(0xffffffffu, x[i], other), cs = s_cos[k][e + i], sn = s_sin[k][e + i];
+                    if (first) x[i] = x[i] * cs - y * sn;
+                    else if (second) x[i] = x[i] * cs + y * sn;
                 }
             }
         }
-        if (is_q) {
+        if (is_q)
             store_lane<CH>(q_out + (size_t)r * ld_q + (size_t)slot * d + lane * CH, x);
-        } else {
-            const int64_t cr = row_index(cache, seq, is_v ? slot - hq - hkv : slot - hq, start + t);
-            store_cache_row<CH>(cache, is_v, cr, lane, x);
-        }
+        else
+            store_cache_row<CH>(cache, is_v, row_index(cache, seq, is_v ? slot - hq - hkv : slot - hq, start + t), lane, x);
     }
 }
 
@@ -383,19 +385,24 @@ extern "C" int dflash_stack_attn_prep_batch(const dflash_bf16* qkv, long long ld
                     "aligned", who);
     int dev = 0;
     DFLASH_CUDA_TRY(cudaGetDevice(&dev));
-    const long long items = (long long)cache->sequences * tokens * (hq + 2 * hkv);
-    const long long blocks = (items + 7) / 8, most = 8ll * sm_count(dev);
-    const dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most)), block(kv::kPrepThreads);
+    // many rows: eight of them and all their heads per CTA, whose cosines are then made once; few: a row and eight
+    // heads per CTA, a head per warp (8 rows x 32 heads: 4.7 us against 9 with all heads in a CTA)
+    const long long rows = (long long)cache->sequences * tokens;
+    const int slots = hq + 2 * hkv;
+    const bool many = rows * slots >= 64ll * sm_count(dev);
+    const int rows_per = many ? kv::kPrepRows : 1, slots_per = many ? slots : kv::kPrepThreads / 32;
+    const dim3 grid(static_cast<unsigned>((rows + rows_per - 1) / rows_per), (slots + slots_per - 1) / slots_per),
+        block(kv::kPrepThreads);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const kv::View c = kv::view_of(*cache);
     cudaError_t e;
     switch (d) {
         case 64: e = launch_chained(kv::attn_prep_batch_kernel<2>, grid, block, 0, s, 1, qkv, ld, q_norm, k_norm, q_out,
-                                    ld_q, c, lengths, tokens, hq, rot, position0, eps, theta, parents); break;
+                                    ld_q, c, lengths, tokens, hq, rot, position0, eps, theta, parents, rows_per, slots_per); break;
         case 128: e = launch_chained(kv::attn_prep_batch_kernel<4>, grid, block, 0, s, 1, qkv, ld, q_norm, k_norm, q_out,
-                                     ld_q, c, lengths, tokens, hq, rot, position0, eps, theta, parents); break;
+                                     ld_q, c, lengths, tokens, hq, rot, position0, eps, theta, parents, rows_per, slots_per); break;
         default: e = launch_chained(kv::attn_prep_batch_kernel<8>, grid, block, 0, s, 1, qkv, ld, q_norm, k_norm, q_out,
-                                    ld_q, c, lengths, tokens, hq, rot, position0, eps, theta, parents);
+                                    ld_q, c, lengths, tokens, hq, rot, position0, eps, theta, parents, rows_per, slots_per);
     }
     DFLASH_CUDA_TRY(e);
     return DFLASH_OK;

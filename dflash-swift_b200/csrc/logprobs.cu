@@ -38,6 +38,12 @@ struct Vec {  // a 16-byte load of logits
         if constexpr (N == 8) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
         else return __uint_as_float(w[i]);
     }
+    __device__ __forceinline__ float pick(int i) const {  // at() for an index that is not a constant
+        const int k = N == 8 ? i >> 1 : i;
+        const uint32_t w = k & 2 ? (k & 1 ? u.w : u.z) : (k & 1 ? u.y : u.x);
+        if constexpr (N == 8) return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+        else return __uint_as_float(w);
+    }
     __device__ __forceinline__ void hide() {  // -inf everywhere: counts as nothing
         const uint32_t v = N == 8 ? 0xff80ff80u : 0xff800000u;
         u = make_uint4(v, v, v, v);
@@ -240,9 +246,15 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
                 const int i = v0 + (r * kUnroll + u) * kThreads + tid;
-                if (peak[u] >= reach && i < v1) {  // seldom: the elements are read again
-#pragma unroll 1
-                    for (int e = lead + i * N; e < lead + i * N + N; ++e) collect(scalar(x + e), e);
+                if (peak[u] >= reach && i < v1) {  // seldom
+                    uint32_t found = 0;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) found |= (v[u].at(e) >= reach ? 1u : 0u) << e;
+                    while (found) {
+                        const int e = __ffs(found) - 1;
+                        found &= found - 1;
+                        collect(v[u].pick(e), lead + i * N + e);
+                    }
                 }
             }
             __syncthreads();

@@ -827,6 +827,12 @@ def _elsewhere(device, stream):
     return None
 
 
+def _current_stream() -> int:
+    """The current device's current stream, without the Stream object that torch.cuda.current_stream() makes."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
 def _rows_bf16(name, t, device, cols=None):
     """Checks rows of bf16 whose elements are adjacent."""
     import torch
@@ -881,7 +887,7 @@ def stack_attn_prep_batch(qkv, q_norm, k_norm, cache: KVCache, lengths, hq: int,
             raise ValueError(f"q_out {tuple(q_out.shape)} for {qkv.shape[0]} rows of {hq * d}")
     check(lib.dflash_stack_attn_prep_batch(_ptr(qkv), qkv.stride(0), _ptr(q_norm), _ptr(k_norm), _ptr(q_out),
                                            q_out.stride(0), cache.ref, _ptr(lengths), T, hq, rot, position0, eps, theta,
-                                           _ptr(parents), _stream()))
+                                           _ptr(parents), _current_stream()))
     return q_out
 
 
@@ -927,7 +933,7 @@ def stack_attn_decode_batch(q, cache: KVCache, lengths, scale: float, out=None, 
     check(lib.dflash_stack_attn_decode_batch(
         _ptr(q), q.stride(0), _ptr(gate), 0 if gate is None else gate.stride(0), cache.ref, _ptr(lengths),
         None if prefix is None else prefix.ref, prefix_len, _ptr(out), T, hq, scale, _ptr(parents),
-        _ptr(workspace), workspace.numel() * workspace.element_size(), _stream()))
+        _ptr(workspace), workspace.numel() * workspace.element_size(), _current_stream()))
     return out
 
 
@@ -948,7 +954,7 @@ def stack_kv_read(cache: KVCache, rows: int, starts=None, k=None, v=None, stream
         _ints("starts", starts, cache.device, (cache.sequences,))
     k, v = (torch.empty(shape, dtype=torch.bfloat16, device=cache.device) if t is None else t for t in (k, v))
     _cache_rows(k, v, shape, cache.device)
-    check(lib.dflash_stack_kv_read(cache.ref, _ptr(starts), rows, _ptr(k), _ptr(v), _stream()))
+    check(lib.dflash_stack_kv_read(cache.ref, _ptr(starts), rows, _ptr(k), _ptr(v), _current_stream()))
     return k, v
 
 
@@ -970,7 +976,7 @@ def stack_kv_write(cache: KVCache, k, v, starts=None, stream=None):
     _cache_rows(k, v, (cache.sequences, cache.kv_heads, k.shape[2], cache.head_dim), cache.device)
     if starts is not None:
         _ints("starts", starts, cache.device, (cache.sequences,))
-    check(lib.dflash_stack_kv_write(cache.ref, _ptr(starts), k.shape[2], _ptr(k), _ptr(v), _stream()))
+    check(lib.dflash_stack_kv_write(cache.ref, _ptr(starts), k.shape[2], _ptr(k), _ptr(v), _current_stream()))
 
 
 def stack_kv_compact_batch(cache: KVCache, lengths, rows, counts, stream=None):
@@ -983,7 +989,7 @@ def stack_kv_compact_batch(cache: KVCache, lengths, rows, counts, stream=None):
     _ints("lengths", lengths, cache.device, (cache.sequences,))
     _ints("counts", counts, cache.device, (cache.sequences,))
     _ints("rows", rows, cache.device, (cache.sequences, rows.shape[-1]))
-    check(lib.dflash_stack_kv_compact_batch(cache.ref, _ptr(lengths), _ptr(rows), _ptr(counts), rows.shape[1], _stream()))
+    check(lib.dflash_stack_kv_compact_batch(cache.ref, _ptr(lengths), _ptr(rows), _ptr(counts), rows.shape[1], _current_stream()))
 
 
 LOGITS_BF16, LOGITS_FP32 = 0, 1
@@ -1012,7 +1018,7 @@ def logprobs(logits, tokens=None, top: int = 0, stream=None) -> dict:
     ids = torch.empty((rows, top), dtype=torch.int32, device=dev)
     check(lib.dflash_logprobs(_ptr(logits), LOGITS_BF16 if logits.dtype == torch.bfloat16 else LOGITS_FP32,
                               logits.stride(0) if rows > 1 else vocab, rows, vocab, _ptr(tokens), n, top, _ptr(logp),
-                              _ptr(entropy), _ptr(ids), _ptr(best), _stream()))
+                              _ptr(entropy), _ptr(ids), _ptr(best), _current_stream()))
     return {"logprobs": logp, "entropy": entropy, "top_ids": ids, "top_logprobs": best}
 
 
