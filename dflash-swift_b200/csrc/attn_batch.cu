@@ -40,9 +40,10 @@ constexpr int kBox = kKeys * 128;          // bytes of a box: 128 keys x 64 elem
 constexpr int kSoftmaxWarps = 8, kProducerWarps = 8;  // producers: this many for K and as many for V
 constexpr int kIssueWarp = kSoftmaxWarps + 2 * kProducerWarps;
 constexpr int kThreads = 32 * (kIssueWarp + 4);  // whole warpgroups: registers move between them
-// Registers a thread.  The block starts with kThreads x 72 = 64512; the issuing warpgroup gives 32 x 128 = 4096 and the
-// softmax takes 16 x 256 = 4096, so nobody waits for good.  The producers keep theirs.
-constexpr int kSoftmaxRegs = 88, kIssueRegs = 40;
+// Registers a thread.  The block starts with kThreads x 72 = 64512; what the softmax takes is no more than the others
+// give, so nobody waits for good: 256 x 104 + 512 x 64 + 128 x 40 = 64512 over quantised caches (256 x 88 + 512 x 72 +
+// 128 x 40 for 4 bits of 128 dims, whose producers spill under 72) and 256 x 136 + 512 x 48 + 128 x 40 over bf16 ones.
+constexpr int kIssueRegs = 40;
 constexpr int kMaxCtas = 160;              // partials are sized for this many CTAs
 constexpr int kMaxSlots = 10;              // ring slots: two boxes each, one where d is 64
 constexpr int kMaxStages = 8;              // staging slots for codes: 64 or 128 rows each
@@ -144,16 +145,16 @@ struct Unit {
 };
 
 __device__ __forceinline__ int own_keys(const Args& a, int len, int block) {
-    const int last = min(a.tokens * a.G, (block + 1) * a.rb) - 1;
-    return a.parents ? len + a.tokens : len + last / a.G + 1;
+    if (a.parents || block + 1 == a.blocks_o) return len + a.tokens;
+    return len + ((block + 1) * a.rb - 1) / a.G + 1;
 }
 __device__ __forceinline__ int live_length(const Args& a, int seq) {
     const int n = a.lengths[seq];
     return n > a.cache.max_len - a.tokens ? -1 : n;
 }
 __device__ __forceinline__ int entry_tiles(const Args& a, int e) {
-    const int len = live_length(a, e / a.blocks_o);
-    return len < 0 ? 0 : (own_keys(a, len, e % a.blocks_o) + kKeys - 1) / kKeys;
+    const int seq = a.blocks_o == 1 ? e : e / a.blocks_o, len = live_length(a, seq);  // most often one block: no division
+    return len < 0 ? 0 : (own_keys(a, len, e - seq * a.blocks_o) + kKeys - 1) / kKeys;
 }
 
 struct Walker {
@@ -167,7 +168,7 @@ struct Walker {
             u.prefix = true;
             u.segment = s;
             u.block = s / a.cache.hkv;
-            u.head = s % a.cache.hkv;
+            u.head = s - u.block * a.cache.hkv;
             u.seq = 0;
             u.tiles = tiles_p;
             u.t0 = w - s * tiles_p;
@@ -182,8 +183,8 @@ struct Walker {
             const int rel = w - off;
             u.prefix = false;
             u.head = rel / tiles;
-            u.seq = entry / a.blocks_o;
-            u.block = entry % a.blocks_o;
+            u.seq = a.blocks_o == 1 ? entry : entry / a.blocks_o;
+            u.block = entry - u.seq * a.blocks_o;
             u.segment = (long long)entry * a.cache.hkv + u.head;
             u.tiles = tiles;
             u.t0 = rel - u.head * tiles;
@@ -289,6 +290,8 @@ struct Kernel {
     // Keys are scaled to 2^kTop .. 2^(kTop + 1): the step of a group, at most 2^(kTop + 2) / (2^BITS - 1), has
     // to stay under 2^-8 (store_groups).
     static constexpr int kTop = BITS == 8 ? -3 : -7;
+    static constexpr int kProducerRegs = BITS == 16 ? 48 : BITS == 4 && D == 128 ? 72 : 64;
+    static constexpr int kSoftmaxRegs = (64512 - 128 * kIssueRegs - 512 * kProducerRegs) / 256;
     static constexpr int NB = D / 64;                  // boxes of a K or V tile
     static constexpr int MB = D > 64 ? D / 128 : 1;    // 128-lane blocks of O^T (half used when d is 64) = ring slots of a tile
     static constexpr int kSub = NB / MB, kSlot = kSub * kBox;  // boxes and bytes of a ring slot
@@ -731,7 +734,7 @@ struct Kernel {
     __device__ static __forceinline__ void load_q(const Args& a, const Unit& u) {
         constexpr int kPer = D / 8, kBatch = 4;  // 16-byte pieces of a row, which sit in one warp; loads in flight
         const int tid = threadIdx.x;
-        const int t0 = u.block * a.rb / a.G, g0 = u.block * a.rb - t0 * a.G;
+        const int t0 = u.block ? u.block * a.rb / a.G : 0, g0 = u.block * a.rb - t0 * a.G;
         const uint16_t* base = a.q + ((u.prefix ? 0 : (int64_t)u.seq * a.tokens) + t0) * a.ld_q + (size_t)u.head * a.G * D;
         // row n of the block is token t0 + v / G, head v % G of v = g0 + n < 256: a product with 2^16 / G
         const auto token_of = [&](int n) { return static_cast<int>(static_cast<uint32_t>((g0 + n) * a.g_magic) >> 16); };
@@ -1075,6 +1078,7 @@ struct Kernel {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             softmax(a, w, tmem, blockIdx.x);
         } else if (warp < kIssueWarp) {
+            if constexpr (kProducerRegs < 72) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
             if constexpr (kQuant) produce_quant(a, w, warp >= kSoftmaxWarps + kProducerWarps);
             else produce_bf16(a, w);
         } else {
@@ -1102,19 +1106,23 @@ __device__ __forceinline__ float element(const kv::View& c, int64_t row, int e) 
     return fmaf(bf16_bits_to_float(c.vs[g]), static_cast<float>(code), bf16_bits_to_float(c.vb[g]));
 }
 
-// Joins the partials of a row and applies the gate: one warp per (row, q head).
+// Joins the partials of a row and applies the gate.  `ways` warps of a CTA share a (row, q head): all eight
+// where that leaves few CTAs idle, one where there are rows enough (the reads of a partial are one dependent
+// chain of a few hundred nanoseconds each otherwise: 37 partials of 192 rows).
 template <int BITS, int D>
-__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ Args a) {
-    constexpr int CH = D / 32;
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ Args a, int ways) {
+    constexpr int CH = D / 32, kWarps = 8;
+    __shared__ float s_m[kWarps], s_l[kWarps], s_acc[kWarps][D];
+    __shared__ int s_poison[kWarps];
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (item >= (long long)a.cache.sequences * a.tokens * a.hq) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, way = ways == 1 ? 0 : warp;
+    const long long item = ways == 1 ? (long long)blockIdx.x * kWarps + warp : blockIdx.x;
+    if (item >= (long long)a.cache.sequences * a.tokens * a.hq) return;  // whole warps, and where ways is 8 never
     const int r = static_cast<int>(item / a.hq), h = static_cast<int>(item - (long long)r * a.hq);
     const int seq = r / a.tokens, t = r - seq * a.tokens, head = h / a.G, g = h - head * a.G;
     const int len = live_length(a, seq);
-    if (len < 0) return;
+    if (len < 0) return;  // every warp of the item
     float m = -INFINITY, l = 0.f, acc[CH];
     int poison = 0;
 #pragma unroll
@@ -1123,13 +1131,13 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
         const bool prefix = side == 0;
         if (prefix && a.blocks_p == 0) continue;
         const long long row = prefix ? (long long)r * a.G + g : (long long)t * a.G + g;
-        const int block = static_cast<int>(row / a.rb), n = static_cast<int>(row % a.rb);
+        const int block = static_cast<int>(row / a.rb), n = static_cast<int>(row - (long long)block * a.rb);
         const long long seg = prefix ? (long long)block * a.cache.hkv + head
                                      : ((long long)seq * a.blocks_o + block) * a.cache.hkv + head;
         const long long meta = (prefix ? 0 : segments_p(a)) + seg;
-        const int c0 = a.first[meta], c1 = a.last[meta];
-        for (int base = c0; base <= c1; base += 32) {
-            const int mine = base + lane;
+        const int c0 = a.first[meta] + way, c1 = a.last[meta];
+        for (int base = c0; base <= c1; base += 32 * ways) {
+            const int mine = base + lane * ways;
             float2 ml = make_float2(-INFINITY, 0.f);
             if (mine <= c1) {
                 ml = a.ml[partial_row(a, prefix, seg, mine) + n];
@@ -1146,13 +1154,13 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
             l = fmaf(w, ml.y, l);  // summed over the lanes below
 #pragma unroll
             for (int i = 0; i < CH; ++i) acc[i] *= old;
-            const int count = min(32, c1 - base + 1);
+            const int count = min(32, (c1 - base) / ways + 1);
             for (int j0 = 0; j0 < count; j0 += 4) {
                 float x[4][CH];
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
                     if (j0 + u < count) {
-                        const float* src = a.o + (partial_row(a, prefix, seg, base + j0 + u) + n) * D + lane * CH;
+                        const float* src = a.o + (partial_row(a, prefix, seg, base + (j0 + u) * ways) + n) * D + lane * CH;
 #pragma unroll
                         for (int i = 0; i < CH; i += 2) {
                             const float2 v = *reinterpret_cast<const float2*>(src + i);
@@ -1174,6 +1182,33 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     poison = __any_sync(0xffffffffu, poison != 0);
+    if (ways > 1) {  // the warps' parts, in order
+        if (lane == 0) {
+            s_m[warp] = m;
+            s_l[warp] = l;
+            s_poison[warp] = poison;
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) s_acc[warp][lane * CH + i] = acc[i];
+        __syncthreads();
+        if (warp != 0) return;
+        poison = 0;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) poison |= s_poison[k];
+        float mx = s_m[0];
+#pragma unroll
+        for (int k = 1; k < kWarps; ++k) mx = fmaxf(mx, s_m[k]);
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+            const float w = s_m[k] == -INFINITY ? 0.f : ex2(s_m[k] - mx);
+            l = fmaf(w, s_l[k], l);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) acc[i] = fmaf(w, s_acc[k][lane * CH + i], acc[i]);
+        }
+    }
     const float inv = (BITS == 16 ? 1.f : exp2i(-Kernel<BITS, D>::kTop)) / l;
 #pragma unroll
     for (int i = 0; i < CH; ++i) acc[i] *= inv;
@@ -1298,7 +1333,9 @@ static cudaError_t launch(const Args& a, int ctas, cudaStream_t s) {
     e = launch_chained(attn_batch_kernel<BITS, D>, dim3(ctas), dim3(kThreads), a.l.total, s, 1, a);
     if (e != cudaSuccess) return e;
     const long long items = (long long)a.cache.sequences * a.tokens * a.hq;
-    return launch_chained(attn_join_kernel<BITS, D>, dim3(static_cast<unsigned>((items + 7) / 8)), dim3(256), 0, s, 1, a);
+    const int ways = items <= 8ll * ctas ? 8 : 1;
+    return launch_chained(attn_join_kernel<BITS, D>, dim3(static_cast<unsigned>(ways == 1 ? (items + 7) / 8 : items)), dim3(256), 0,
+                          s, 1, a, ways);
 }
 
 }  // namespace attn
