@@ -19,11 +19,11 @@
 // key's values (and every query row) are first scaled by a power of two into fp16's upper range,
 // undone in S^T for K and Q, and for V folded into P's exponent and the sum's weights.
 //
-// Roles: warps 0-7 softmax (two per TMEM lane quarter, half of the columns each), 8-15 producers of K
-// and 16-23 of V (cache rows to swizzled shared memory boxes of 128 keys x 64 elements, in a ring),
-// warp 24 issues the products, warps 25 and 26 the bulk copies of K's and V's codes to staging
-// slots (27 has no work).  The running maximum is only raised when a score passes it by kLazy (in powers
-// of two), so the accumulators are rarely rescaled.
+// Roles: first the softmax warps (per TMEM lane quarter two or four, 32 columns each), then the producers (cache
+// rows to swizzled shared memory boxes of 128 keys x 64 elements, in rings; over quantised caches half of
+// them for K and half for V), warp 24 issues the products, warps 25 and 26 the bulk copies of K's and V's
+// codes to staging slots (27 has no work).  The running maximum is only raised when a score passes it by
+// kLazy (in powers of two), so the accumulators are rarely rescaled.
 #include "common.cuh"
 #include "dflash_batch.h"
 #include "tcgen05.cuh"
@@ -37,13 +37,11 @@ namespace attn {
 constexpr int kKeys = 128;
 constexpr int kRows = 128;
 constexpr int kBox = kKeys * 128;          // bytes of a box: 128 keys x 64 elements of 16 bits
-constexpr int kSoftmaxWarps = 8, kProducerWarps = 8;  // producers: this many for K and as many for V
-constexpr int kIssueWarp = kSoftmaxWarps + 2 * kProducerWarps;
+constexpr int kIssueWarp = 24;             // behind the softmax and producer warps, 8 of one and 16 of the other
 constexpr int kThreads = 32 * (kIssueWarp + 4);  // whole warpgroups: registers move between them
-// Registers a thread.  The block starts with kThreads x 72 = 64512; what the softmax takes is no more than the others
-// give, so nobody waits for good: 256 x 104 + 512 x 64 + 128 x 40 = 64512 over quantised caches (256 x 88 + 512 x 72 +
-// 128 x 40 for 4 bits of 128 dims, whose producers spill under 72) and 256 x 136 + 512 x 48 + 128 x 40 over bf16 ones.
-constexpr int kIssueRegs = 40;
+// Registers a thread at launch, and behind setmaxnreg for the issuing warpgroup; the producers give too, and what the
+// softmax takes is no more than that, so nobody waits for good.
+constexpr int kLaunchRegs = 72, kIssueRegs = 40;
 constexpr int kMaxCtas = 160;              // partials are sized for this many CTAs
 constexpr int kMaxSlots = 10;              // ring slots: two boxes each, one where d is 64
 constexpr int kMaxStages = 8;              // staging slots for codes: 64 or 128 rows each
@@ -54,6 +52,7 @@ constexpr float kLift = 8.f;               // ... and P is 2^8 p, up to 2^12: sm
 constexpr float kNever = 1e30f;            // base of a row without a maximum yet: every score passes it
 constexpr int kTopQ = 12;                  // query rows are scaled to 2^12 .. 2^13 in fp16
 constexpr uint32_t kTmemColumns = 512;
+constexpr int kAllSoftmax = 5;               // named barrier of all softmax warps; 1 to 4: of those with the same columns
 constexpr int kSmemLimit = 232448;
 
 // Shared memory: what has a fixed size first, so that its addresses are constants; then the scale
@@ -290,8 +289,14 @@ struct Kernel {
     // Keys are scaled to 2^kTop .. 2^(kTop + 1): the step of a group, at most 2^(kTop + 2) / (2^BITS - 1), has
     // to stay under 2^-8 (store_groups).
     static constexpr int kTop = BITS == 8 ? -3 : -7;
-    static constexpr int kProducerRegs = BITS == 16 ? 48 : BITS == 4 && D == 128 ? 72 : 64;
-    static constexpr int kSoftmaxRegs = (64512 - 128 * kIssueRegs - 512 * kProducerRegs) / 256;
+    // 16 softmax warps, four per TMEM lane quarter with 32 columns each, and 8 producers; over quantised caches of 256
+    // dims, whose row blocks have 64 rows and whose codes take twice the unpacking, 8 and 16.
+    static constexpr int kSoftmaxWarps = kQuant && D == 256 ? 8 : 16, kSubs = kSoftmaxWarps / 4;
+    static constexpr int kProducerWarps = kIssueWarp - kSoftmaxWarps;
+    static constexpr int kGroupWarps = kQuant ? kProducerWarps / 2 : kProducerWarps, kGroup = 32 * kGroupWarps;  // that fill a box
+    static constexpr int kProducerRegs = kQuant ? kSoftmaxWarps == 8 ? 64 : 72 : 48;
+    static constexpr int kSoftmaxRegs =
+        (32 * (28 * kLaunchRegs - 4 * kIssueRegs - kProducerWarps * kProducerRegs) / (32 * kSoftmaxWarps)) / 8 * 8;
     static constexpr int NB = D / 64;                  // boxes of a K or V tile
     static constexpr int MB = D > 64 ? D / 128 : 1;    // 128-lane blocks of O^T (half used when d is 64) = ring slots of a tile
     static constexpr int kSub = NB / MB, kSlot = kSub * kBox;  // boxes and bytes of a ring slot
@@ -366,10 +371,10 @@ struct Kernel {
     }
 
     // The pieces of a box that a producer thread writes: kPieces rows, kChunks 16-byte chunks of each.
-    static constexpr int kGroup = kQuant ? 32 * kProducerWarps : 64 * kProducerWarps;  // threads that fill a box
-    static constexpr int kPieces = kQuant ? BITS / 4 : 2, kChunks = kQuant ? 16 / BITS : 1;
+    static constexpr int kChunks = kQuant ? 16 / BITS : 1;
     static constexpr int kRowThreads = kQuant ? BITS / 2 : 8;  // threads that share a row
-    __device__ static __forceinline__ int piece_key(int pt, int u) { return pt / kRowThreads + u * (kGroup / kRowThreads); }
+    static constexpr int kRowStep = kGroup / kRowThreads, kPieces = kKeys / kRowStep;
+    __device__ static __forceinline__ int piece_key(int pt, int u) { return pt / kRowThreads + u * kRowStep; }
 
     // A non-finite element of a row that some query row does not see would reach it as 0 * inf: it is
     // taken out of the operand and the unit's flag raised, for the join to put it back where it is
@@ -417,11 +422,11 @@ struct Kernel {
                     wait(&fixed().empty[ring.slot], ring.phase ^ 1);
 #pragma unroll
                     for (int x = 0; x < kPieces; ++x) {
-                        const bool live = key0 + 64 * x < valid;
+                        const bool live = key0 + kRowStep * x < valid;
 #pragma unroll
                         for (int y = 0; y < kSub; ++y)
-                            cp_async16(dst0 + ring.slot * kSlot + y * kBox + x * 64 * 128,
-                                       live ? p + x * (64 * D * 2) + y * 128 : src.k, live);
+                            cp_async16(dst0 + ring.slot * kSlot + y * kBox + x * kRowStep * 128,
+                                       live ? p + x * (kRowStep * D * 2) + y * 128 : src.k, live);
                     }
                     if (__builtin_expect(is_v && look < valid, 0)) {
                         cp_async_wait_all();
@@ -466,7 +471,8 @@ struct Kernel {
         }
     }
 
-    // Scales and biases of one key, as raw bf16 pairs: up to two words of each, of four, for one lane.
+    // Scales and biases of one key, as raw bf16 pairs: up to two words of each, of four where a key has
+    // eight groups (256 dims) and two lanes, for one lane.
     struct Groups {
         uint32_t s[2], b[2];
     };
@@ -486,7 +492,7 @@ struct Kernel {
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                if (2 * (first + i) < groups && (i == 0 || groups == 8)) {
+                if (2 * (first + i) < groups && (i == 0 || groups == 8 || kGroupWarps == 4)) {
                     g.s[i] = reinterpret_cast<const uint32_t*>(ps)[first + i];
                     g.b[i] = reinterpret_cast<const uint32_t*>(pb)[first + i];
                 }
@@ -516,7 +522,7 @@ struct Kernel {
         const float f24 = f * 16777216.f;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (2 * (first + i) < groups && (i == 0 || groups == 8)) {
+            if (2 * (first + i) < groups && (i == 0 || groups == 8 || kGroupWarps == 4)) {
                 const uint32_t e0 = pack2<false>(__uint_as_float(g.s[i] << 16) * f24, __uint_as_float(g.b[i] << 16) * f);
                 asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr + 8 * (first + i)), "r"(e0) : "memory");
                 if (groups > 1) {
@@ -549,7 +555,7 @@ struct Kernel {
     }
 
     __device__ static void produce_quant(const Args& a, Walker w, bool is_v) {
-        const int pt = threadIdx.x & (32 * kProducerWarps - 1), groups = D / a.cache.group;
+        const int pt = threadIdx.x & (kGroup - 1), groups = D / a.cache.group;
         const int piece = pt % kRowThreads, key0 = pt / kRowThreads;
         const uint32_t ring_at = smem_at(a.l.ring), slot_bytes = a.stage_rows * (D * BITS / 8);
         const int shift = 31 - __clz(a.cache.group);
@@ -562,10 +568,11 @@ struct Kernel {
         for (int i = 0; i < kChunks; ++i) chunk[i] = key0 * 128 + (((kChunks * piece + i) ^ (key0 & 7)) << 4);
         const uint32_t from = smem_at(a.l.stage) + key0 * kRowBytes + piece * 16;
         const bool halves = a.stage_rows < kKeys;
-        // Scales: a warp unpacks the same 16 keys of every tile, so it keeps their tables for itself, two lanes a key.
+        // Scales: a warp unpacks the same keys of every tile, so it keeps their tables for itself, one or two lanes a key.
         // V's are made a tile ahead of its unpacking, since the softmax needs V's factor.
-        const int lane = threadIdx.x & 31, kk = lane & 15, first = groups == 8 ? 2 * (lane >> 4) : lane >> 4;
-        const int key_of = (pt >> 5) * (BITS == 8 ? 8 : 16) + (BITS == 8 ? (kk & 7) + 64 * (kk >> 3) : kk);
+        constexpr int kOwn = kKeys / kGroupWarps, kRun = 32 / kRowThreads;  // keys of a warp, in runs of kRun
+        const int lane = threadIdx.x & 31, kk = lane % kOwn, first = groups == 8 ? 2 * (lane / kOwn) : lane / kOwn;
+        const int key_of = (pt >> 5) * kRun + kk % kRun + kk / kRun * kRowStep;
         const uint32_t table_bytes = kKeys * groups * 4, tables = smem_at(kTables) + (is_v ? table_bytes : 0);
         Groups g;
         Ring ring = ring_of(a, is_v);
@@ -574,10 +581,10 @@ struct Kernel {
         uint32_t phase = 0;
         // look: first row of the tile to look at for non-finite values, kKeys for none
         const auto emit = [&](uint32_t table, int look, int unit) {
-            uint32_t codes[kPieces];  // kPieces x (kGroup / kRowThreads) rows: one slot, or two halves
-            int staged[kPieces];
+            uint32_t codes[2];  // the tile's rows 0 and 64 on: one slot, or two halves
+            int staged[2];
 #pragma unroll
-            for (int x = 0; x < kPieces; ++x) {
+            for (int x = 0; x < 2; ++x) {
                 if (x == 0 || halves) {
                     staged[x] = slot;
                     codes[x] = from + slot * slot_bytes;
@@ -587,7 +594,7 @@ struct Kernel {
                         phase ^= 1;
                     }
                 } else {
-                    codes[x] = codes[0] + x * (kGroup / kRowThreads) * kRowBytes;
+                    codes[x] = codes[0] + kKeys / 2 * kRowBytes;
                 }
             }
             const uint32_t entry = table + key0 * groups * 4;
@@ -601,8 +608,8 @@ struct Kernel {
                     const uint32_t sb = entry + ((box * 64 + piece * (128 / BITS)) >> shift) * 4;
 #pragma unroll
                     for (int x = 0; x < kPieces; ++x)
-                        unpack(lds128(codes[x] + box * (8 * BITS)), lds32(sb + x * (kGroup / kRowThreads) * groups * 4),
-                               box0 + mine * kBox + x * (kGroup / kRowThreads) * 128, chunk);
+                        unpack(lds128(codes[x * kRowStep / 64] + x * kRowStep % 64 * kRowBytes + box * (8 * BITS)), lds32(sb + x * kRowStep * groups * 4),
+                               box0 + mine * kBox + x * kRowStep * 128, chunk);
                 }
                 if (__builtin_expect(look < kKeys, 0))
 #pragma unroll 1
@@ -612,7 +619,7 @@ struct Kernel {
             }
             if ((threadIdx.x & 31) == 0) {  // the codes have been read
 #pragma unroll
-                for (int x = 0; x < kPieces; ++x)
+                for (int x = 0; x < 2; ++x)
                     if (x == 0 || halves) mbar_arrive(&fixed().unstaged[staged[x]]);
             }
         };
@@ -632,12 +639,14 @@ struct Kernel {
                     const int depth = tile % kScaleDepth;
                     wait(&fixed().sc_empty[depth], ((tile / kScaleDepth) & 1) ^ 1);
                     float top = largest(g);
-                    const float other = __shfl_xor_sync(0xffffffffu, top, 16);
-                    asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(other));
+                    if constexpr (kOwn == 16) {
+                        const float other = __shfl_xor_sync(0xffffffffu, top, 16);
+                        asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(other));
+                    }
                     const int e = min(max(exponent(top), -100), 100);
                     store_groups(tables + (is_v ? (tile & 1) * table_bytes : 0) + key_of * groups * 4, g, groups, first,
                                  exp2i(kTop - e));
-                    if (lane < 16) {
+                    if (lane < kOwn) {
                         if (is_v) {
                             fixed().key_v[depth][key_of] = e;
                         } else {
@@ -790,10 +799,10 @@ struct Kernel {
     }
 
     __device__ static void softmax(const Args& a, Walker w, uint32_t tmem, int cta) {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3, half = warp >> 2;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3, sub = warp >> 2;
         const int key = quarter * 32 + lane, tid = threadIdx.x & 127;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        const int columns = a.nr / 2, c0 = half * columns;  // this warp's columns of S^T
+        const int n0 = sub * 32;  // this warp's 32 columns of S^T
         const float qscale = a.scale * 1.4426950408889634f;
         int tile = 0, units = 0;
         Unit u;
@@ -801,13 +810,14 @@ struct Kernel {
             load_q(a, u);
             fence_proxy_async_shared();
             tc5::fence_before();
-            named_bar_sync(4, 32 * kSoftmaxWarps);
+            named_bar_sync(kAllSoftmax, 32 * kSoftmaxWarps);
             if (threadIdx.x == 0) {
                 fixed().unit_tiles = u.n;
                 fixed().unit_rows = u.rows;
                 mbar_arrive(&fixed().q_full);
             }
-            float l0 = 0.f, l1 = 0.f;  // sums over this warp's keys: lane j has column c0 + j, and c0 + 32 + j
+            const bool live = n0 < u.rows;
+            float sum = 0.f;  // over this warp's keys, lane j has column n0 + j
             for (int i = 0; i < u.n; ++i, ++tile) {
                 const int depth = tile % kScaleDepth;
                 float ks = 1.f, ev = 0.f;
@@ -821,17 +831,15 @@ struct Kernel {
                 const int at = (u.t0 + i) * kKeys;
                 const int b = at + key - u.len;  // block row of the key; a prefix ends where its block would begin
                 const bool masked = at + kKeys > u.len;
-                bool waited = i == 0;  // for the last tile's p V: P and the accumulators are free
-                const int end = min(c0 + columns, u.rows);
                 const float weight = kQuant ? exp2i(-static_cast<int>(ev)) : 1.f;
+                bool waited = i == 0;  // for the last tile's p V: P and the accumulators are free
                 const auto hand_over = [&]() {
                     fence_proxy_async_shared();
                     tc5::fence_before();
-                    named_bar_sync(1 + half, 128);
+                    named_bar_sync(1 + sub, 128);
                     if (tid == 0) mbar_arrive(&fixed().p_full);
                 };
-#pragma unroll 1
-                for (int n0 = c0; n0 < end; n0 += 32) {  // 32 columns at a time in registers
+                if (live) {
                     float y[32];
                     bool raise = false;  // this pass: plain scores for new maxima, not scores relative to the old ones
 #pragma unroll 1
@@ -869,7 +877,7 @@ struct Kernel {
 #pragma unroll
                             for (int j = 4; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], y[j]);
                             if (pass == 0)
-                                raise = bar_any(1 + half, 128,
+                                raise = bar_any(1 + sub, 128,
                                                 fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > kLazy + kLift);
                             if (!waited) {
                                 wait(&fixed().pv_done, (tile - 1) & 1);
@@ -887,7 +895,7 @@ struct Kernel {
                             if (lane == j) mine = m;
                         }
                         fixed().part[quarter][n0 + lane] = mine;
-                        named_bar_sync(1 + half, 128);
+                        named_bar_sync(1 + sub, 128);
                         if (tid < 32 && n0 + tid < u.rows) {
                             const int n = n0 + tid;
                             const float old = fixed().m[n];
@@ -897,7 +905,7 @@ struct Kernel {
                             fixed().m[n] = m;
                             if (m > -INFINITY) fixed().base[n] = kLift - m;
                         }
-                        named_bar_sync(1 + half, 128);
+                        named_bar_sync(1 + sub, 128);
                         if (i > 0 && (D > 64 || quarter < 2)) {  // the accumulators so far go to the new maxima
                             for (int mb = 0; mb < MB; ++mb)
                                 for (int n1 = n0; n1 < min(n0 + 32, u.rows); n1 += 16) {
@@ -912,7 +920,7 @@ struct Kernel {
                                 }
                             tc5::wait_st();
                         }
-                        if (n0 + lane < u.rows) (n0 == c0 ? l0 : l1) *= fixed().corr[n0 + lane];  // and the sums
+                        if (n0 + lane < u.rows) sum *= fixed().corr[n0 + lane];  // and the sums
                     }
                     const uint32_t row = smem_at(a.l.p) + (n0 >> 6) * kBox + key * 128;
 #pragma unroll
@@ -923,14 +931,13 @@ struct Kernel {
                                make_uint4(pack2<!kQuant>(y[j], y[j + 1]), pack2<!kQuant>(y[j + 2], y[j + 3]),
                                           pack2<!kQuant>(y[j + 4], y[j + 5]), pack2<!kQuant>(y[j + 6], y[j + 7])));
                     }
-                    if (n0 + 32 >= end) hand_over();  // before the sums, which nobody waits for
+                    hand_over();  // before the sums, which nobody waits for
                     if (kQuant) {  // V's factor is part of P
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) mul2(y[j], y[j + 1], weight, weight);
                     }
-                    (n0 == c0 ? l0 : l1) += stack::reduce_scatter32(y, lane);
-                }
-                if (c0 >= end) {  // no columns of its own
+                    sum += stack::reduce_scatter32(y, lane);
+                } else {
                     if (i > 0) {
                         wait(&fixed().pv_done, (tile - 1) & 1);
                         tc5::fence_after();
@@ -950,20 +957,19 @@ struct Kernel {
                 for (int mb = 0; mb < MB; ++mb) {
                     const int e = mb * 128 + quarter * 32 + lane;
                     float* o = a.o + at * D + ((e & ~7) | order<BITS>(e & 7));
-                    for (int n0 = c0; n0 < min(c0 + columns, u.rows); n0 += 16) {
+                    for (int n1 = n0; n1 < min(n0 + 32, u.rows); n1 += 16) {
                         uint32_t r[16];
-                        tc5::ld16(tmem + lanes + (2 + mb) * a.nr + n0, r);
+                        tc5::ld16(tmem + lanes + (2 + mb) * a.nr + n1, r);
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
-                            if (n0 + j < u.rows) o[(long long)(n0 + j) * D] = __uint_as_float(r[j]);
+                            if (n1 + j < u.rows) o[(long long)(n1 + j) * D] = __uint_as_float(r[j]);
                     }
                 }
             }
-            if (c0 + lane < u.rows) fixed().part[quarter][c0 + lane] = l0;
-            if (columns > 32 && c0 + 32 + lane < u.rows) fixed().part[quarter][c0 + 32 + lane] = l1;
-            named_bar_sync(1 + half, 128);
-            if (tid < columns && c0 + tid < u.rows) {
-                const int n = c0 + tid;
+            if (live) fixed().part[quarter][n0 + lane] = sum;
+            named_bar_sync(1 + sub, 128);
+            if (tid < 32 && n0 + tid < u.rows) {
+                const int n = n0 + tid;
                 a.ml[at + n] = make_float2(fixed().m[n], (fixed().part[0][n] + fixed().part[1][n]) +
                                                              (fixed().part[2][n] + fixed().part[3][n]));
             }
@@ -977,7 +983,7 @@ struct Kernel {
             }
             ++units;
             tc5::fence_before();
-            named_bar_sync(4, 32 * kSoftmaxWarps);  // Q, the row arrays and the accumulators are free
+            named_bar_sync(kAllSoftmax, 32 * kSoftmaxWarps);  // Q, the row arrays and the accumulators are free
         }
         if (threadIdx.x == 0) {
             fixed().unit_tiles = 0;
@@ -1045,21 +1051,21 @@ struct Kernel {
         const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
         if (threadIdx.x == 0) {
             for (int i = 0; i < kMaxSlots; ++i) {
-                mbar_init(&fixed().full[i], kQuant ? kProducerWarps : kGroup);
+                mbar_init(&fixed().full[i], kQuant ? kGroupWarps : kGroup);
                 mbar_init(&fixed().empty[i], 1);
             }
             mbar_init(&fixed().s_full[0], 1);
             mbar_init(&fixed().s_full[1], 1);
-            mbar_init(&fixed().p_full, 2);
+            mbar_init(&fixed().p_full, kSubs);
             mbar_init(&fixed().pv_done, 1);
             mbar_init(&fixed().q_full, 1);
             for (int i = 0; i < kScaleDepth; ++i) {
-                mbar_init(&fixed().sc_full[i], 2 * kProducerWarps);
+                mbar_init(&fixed().sc_full[i], kProducerWarps);
                 mbar_init(&fixed().sc_empty[i], kSoftmaxWarps);
             }
             for (int i = 0; i < kMaxStages; ++i) {
                 mbar_init(&fixed().staged[i], 1);
-                mbar_init(&fixed().unstaged[i], kProducerWarps);
+                mbar_init(&fixed().unstaged[i], kGroupWarps);
             }
             fixed().abort = 0;
             fence_barrier_init();
@@ -1078,8 +1084,8 @@ struct Kernel {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             softmax(a, w, tmem, blockIdx.x);
         } else if (warp < kIssueWarp) {
-            if constexpr (kProducerRegs < 72) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
-            if constexpr (kQuant) produce_quant(a, w, warp >= kSoftmaxWarps + kProducerWarps);
+            if constexpr (kProducerRegs < kLaunchRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
+            if constexpr (kQuant) produce_quant(a, w, warp >= kSoftmaxWarps + kGroupWarps);
             else produce_bf16(a, w);
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
