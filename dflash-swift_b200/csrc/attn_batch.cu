@@ -49,7 +49,7 @@ constexpr int kScaleDepth = 2;             // tiles whose key factors may be ali
 constexpr int kPoison = 16;                // units whose poison flags may be alive at once
 constexpr float kLazy = 4.f;               // a maximum moves when a score passes it by 2^4 ...
 constexpr float kLift = 8.f;               // ... and P is 2^8 p, up to 2^12: small weights stay normal in fp16
-constexpr float kNever = 1e30f;            // base of a row without a maximum yet: every score passes it
+constexpr float kNever = 3e38f;            // base of a row without a maximum yet: every score passes it
 constexpr int kTopQ = 12;                  // query rows are scaled to 2^12 .. 2^13 in fp16
 constexpr uint32_t kTmemColumns = 512;
 constexpr int kAllSoftmax = 5;               // named barrier of all softmax warps; 1 to 4: of those with the same columns

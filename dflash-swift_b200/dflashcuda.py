@@ -930,6 +930,8 @@ def stack_attn_decode_batch(q, cache: KVCache, lengths, scale: float, out=None, 
     if workspace is None:
         workspace = torch.empty(stack_attn_decode_batch_workspace_bytes(cache, prefix_len, T, hq), dtype=torch.uint8,
                                 device=dev)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace: a contiguous tensor on {dev} is expected")
     check(lib.dflash_stack_attn_decode_batch(
         _ptr(q), q.stride(0), _ptr(gate), 0 if gate is None else gate.stride(0), cache.ref, _ptr(lengths),
         None if prefix is None else prefix.ref, prefix_len, _ptr(out), T, hq, scale, _ptr(parents),
