@@ -97,6 +97,21 @@ __device__ __forceinline__ void store_lane(uint16_t* p, const float (&x)[CH]) {
     else *reinterpret_cast<uint32_t*>(p) = w[0];
 }
 
+// CH consecutive floats from shared memory, aligned as they are long up to 16 bytes.
+template <int CH>
+__device__ __forceinline__ void load_floats(const float* p, float (&x)[CH]) {
+    if constexpr (CH >= 4) {
+#pragma unroll
+        for (int i = 0; i < CH; i += 4) {
+            const float4 u = *reinterpret_cast<const float4*>(p + i);
+            x[i] = u.x; x[i + 1] = u.y; x[i + 2] = u.z; x[i + 3] = u.w;
+        }
+    } else {
+        const float2 u = *reinterpret_cast<const float2*>(p);
+        x[0] = u.x; x[1] = u.y;
+    }
+}
+
 // Quantises the row a warp holds (lane l: elements [l CH, l CH + CH)) in groups of `group`
 // elements = group / CH lanes and writes codes, scales and biases.
 //   edge e: the group's extreme of larger magnitude (the minimum only when strictly larger),
@@ -137,9 +152,26 @@ __device__ __forceinline__ void quantise_row(const float (&x)[CH], int lane, int
         scales[lane / width] = sb;
         biases[lane / width] = bb;
     }
+    // Codes are rint((x - b) / s) of the correctly rounded quotient.  The product with 1 / s is within 255 (2^-24 + 2^-24 +
+    // 2^-24) = 4.6e-5 of it where it matters (further out both are clamped), so wherever it keeps 1e-4 from a tie it
+    // rounds to the same code; a lane with an element nearer, or with a scale whose reciprocal could leave fp32's
+    // normal range, divides.  (4102 rows x 32 heads in 4 bits, with the read-back: 91 us against 96.)
+    const float inverse = 1.f / sr;
+    bool divide = !(fabsf(sr) > 1e-30f && fabsf(sr) < 1e30f);
+    float n[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const float t = (x[i] - br) * inverse;
+        n[i] = rintf(t);
+        divide = divide || !(fabsf(t - n[i]) < 0.4999f);
+    }
+    if (divide && !bad) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) n[i] = rintf((x[i] - br) / sr);
+    }
     uint32_t c[CH];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) c[i] = bad ? 0u : static_cast<uint32_t>(fminf(fmaxf(rintf((x[i] - br) / sr), 0.f), top));
+    for (int i = 0; i < CH; ++i) c[i] = bad ? 0u : static_cast<uint32_t>(fminf(fmaxf(n[i], 0.f), top));
     if (bits == 8) {
         uint8_t* p = codes + lane * CH;
         if constexpr (CH == 8)
@@ -181,7 +213,7 @@ __device__ __forceinline__ void store_cache_row(const View& cache, bool is_v, in
 // position times the frequency's fraction wraps as the angle does, so far positions lose nothing (a
 // float product is off by 2^-24 of the angle, 0.06 rad at a million).  The normalised k stays in 32 bits up
 // to its one rounding, the quantisation.
-constexpr int kPrepThreads = 256, kPrepRows = 8;
+constexpr int kPrepThreads = 256, kPrepRows = 2;
 
 template <int CH>
 __global__ void __launch_bounds__(kPrepThreads) attn_prep_batch_kernel(
@@ -192,6 +224,7 @@ __global__ void __launch_bounds__(kPrepThreads) attn_prep_batch_kernel(
     __shared__ unsigned long long s_turn[d / 2];  // turns per position of pair i, 0.64 fixed point
     __shared__ __align__(16) float s_cos[kPrepRows][d / 2], s_sin[kPrepRows][d / 2];
     __shared__ int s_start[kPrepRows];            // first cache row of the row's block, -1: takes no part
+    __shared__ int s_seq[kPrepRows];
     const int half = rot / 2;
     for (int i = threadIdx.x; i < half; i += kPrepThreads) {
         const double turns = exp2(-2.0 * i / rot * log2(static_cast<double>(theta))) * 0.15915494309189533577;
@@ -200,10 +233,13 @@ __global__ void __launch_bounds__(kPrepThreads) attn_prep_batch_kernel(
     pdl_wait();
     pdl_launch_dependents();
     const int r0 = blockIdx.x * rows_per, rows = min(rows_per, cache.sequences * tokens - r0);
-    if (threadIdx.x < rows) s_start[threadIdx.x] = block_start(lengths, (r0 + threadIdx.x) / tokens, tokens, cache.max_len);
+    if (threadIdx.x < rows) {
+        s_seq[threadIdx.x] = (r0 + threadIdx.x) / tokens;
+        s_start[threadIdx.x] = block_start(lengths, s_seq[threadIdx.x], tokens, cache.max_len);
+    }
     __syncthreads();
     for (int i = threadIdx.x; i < rows * half; i += kPrepThreads) {
-        const int k = i / half, e = i - k * half, seq = (r0 + k) / tokens, t = r0 + k - seq * tokens;
+        const int k = i / half, e = i - k * half, seq = s_seq[k], t = r0 + k - seq * tokens;
         const int depth = parents ? tree_walk(parents + (size_t)seq * tokens, t).depth : t;
         const unsigned long long a = s_turn[e] * static_cast<unsigned long long>((long long)position0 + s_start[k] + depth);
         sincospif(static_cast<float>(static_cast<int>(a >> 32)) * 4.656612873077392578125e-10f, &s_sin[k][e], &s_cos[k][e]);
@@ -216,7 +252,7 @@ __global__ void __launch_bounds__(kPrepThreads) attn_prep_batch_kernel(
     for (int it = threadIdx.x >> 5; it < rows * slots; it += kPrepThreads / 32) {
         const int k = it / slots, slot = slot0 + it - k * slots, start = s_start[k];
         if (start < 0) continue;
-        const int r = r0 + k, seq = r / tokens, t = r - seq * tokens;
+        const int r = r0 + k, seq = s_seq[k], t = r - seq * tokens;
         const bool is_v = slot >= hq + hkv, is_q = slot < hq;
         float x[CH];
         load_lane<CH>(qkv + (size_t)r * ld + (size_t)(is_q ? slot : hq + slot) * d + lane * CH, x);
@@ -233,11 +269,14 @@ __global__ void __launch_bounds__(kPrepThreads) attn_prep_batch_kernel(
             for (int i = 0; i < CH; ++i) x[i] = x[i] * rs * w[i];
             if (rot > 0) {
                 const int e = (second ? lane - pair_lanes : first ? lane : 0) * CH;
+                float cs[CH], sn[CH];
+                load_floats<CH>(&s_cos[k][e], cs);
+                load_floats<CH>(&s_sin[k][e], sn);
 #pragma unroll
                 for (int i = 0; i < CH; ++i) {
-                    const float y = __shfl_sync(0xffffffffu, x[i], other), cs = s_cos[k][e + i], sn = s_sin[k][e + i];
-                    if (first) x[i] = x[i] * cs - y * sn;
-                    else if (second) x[i] = x[i] * cs + y * sn;
+                    const float y = __shfl_sync(0xffffffffu, x[i], other);
+                    if (first) x[i] = x[i] * cs[i] - y * sn[i];
+                    else if (second) x[i] = x[i] * cs[i] + y * sn[i];
                 }
             }
         }
@@ -281,14 +320,13 @@ __global__ void __launch_bounds__(256) kv_read_kernel(View cache, const int32_t*
                                                       uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
     pdl_wait();
     pdl_launch_dependents();
-    const int per_row = cache.d / 8;
-    const long long per_seq = (long long)cache.hkv * rows * per_row, n = per_seq * cache.sequences;
+    const int per_row = cache.d / 8;  // a power of two
+    const long long n = (long long)cache.sequences * cache.hkv * rows * per_row;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const int seq = static_cast<int>(i / per_seq);
-        const long long in_seq = i - seq * per_seq;
-        const int head = static_cast<int>(in_seq / ((long long)rows * per_row));
-        const long long in_head = in_seq - (long long)head * rows * per_row;
-        const int row = static_cast<int>(in_head / per_row), e0 = static_cast<int>(in_head - (long long)row * per_row) * 8;
+        // 2^32 rows of at least 128 bytes of output are more than a GPU has
+        const uint32_t line = static_cast<uint32_t>(i >> (__ffs(per_row) - 1)), of_head = line / rows;
+        const int e0 = static_cast<int>(i & (per_row - 1)) * 8, row = static_cast<int>(line - of_head * rows);
+        const int seq = static_cast<int>(of_head / cache.hkv), head = static_cast<int>(of_head - seq * cache.hkv);
         const int start = starts ? block_start(starts, seq, rows, cache.max_len) : 0;
         if (start < 0) continue;
         const int64_t cr = row_index(cache, seq, head, start + row);
@@ -385,9 +423,9 @@ extern "C" int dflash_stack_attn_prep_batch(const dflash_bf16* qkv, long long ld
                     "aligned", who);
     int dev = 0;
     DFLASH_CUDA_TRY(cudaGetDevice(&dev));
-    // many rows: eight of them and all their heads per CTA, whose cosines are then made once; few: a row and eight
-    // heads per CTA, a head per warp.  With the read-back, 8 rows x 32 heads: 6.9 us as few, 50 as many; 4102 rows:
-    // 100 us as few, 96 as many
+    // many rows: two of them and all their heads per CTA, whose cosines are then made once; few: a row and eight
+    // heads per CTA, a head per warp.  With the read-back, 8 rows x 32 heads: 6.4 us as few, 15 as many; 4102 rows:
+    // 94 us as few, 70 as many (four rows per CTA 77, eight 91: too few warps hide the 1.3 us that a head takes)
     const long long rows = (long long)cache->sequences * tokens;
     const int slots = hq + 2 * hkv;
     const bool many = rows * slots >= 64ll * sm_count(dev);
