@@ -100,7 +100,7 @@ def test_other_argument_errors(dc):
 @pytest.mark.parametrize("kw,status", [
     (dict(x=0), 1), (dict(vocab=0), 1), (dict(rows=-1), 1), (dict(ld=99), 1), (dict(n=-1), 1), (dict(top=-1), 1),
     (dict(tokens=0), 1), (dict(type=2), 2), (dict(top=33), 2), (dict(vocab=7, ld=7, top=8), 2), (dict(x=FAKE + 1), 3),
-    (dict(x=FAKE + 2, type=1), 3), (dict(rows=0), 0),
+    (dict(x=FAKE + 2, type=1), 3), (dict(rows=0), 0), (dict(vocab=2**31 - 100, ld=2**31), 2),
 ])
 def test_logprobs_argument_errors(dc, kw, status):
     a = dict(x=FAKE, type=0, ld=100, rows=4, vocab=100, tokens=FAKE, n=1, top=5)
