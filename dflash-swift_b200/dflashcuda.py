@@ -880,7 +880,7 @@ def stack_attn_prep_batch(qkv, q_norm, k_norm, cache: KVCache, lengths, hq: int,
     if parents is not None:
         _ints("parents", parents, dev, (cache.sequences, T))
     if q_out is None:
-        q_out = torch.empty((qkv.shape[0], hq * d), dtype=torch.bfloat16, device=dev)
+        q_out = qkv.new_empty((qkv.shape[0], hq * d))
     else:
         _rows_bf16("q_out", q_out, dev)
         if q_out.shape[0] != qkv.shape[0] or q_out.shape[1] < hq * d:
@@ -920,7 +920,7 @@ def stack_attn_decode_batch(q, cache: KVCache, lengths, scale: float, out=None, 
     if parents is not None:
         _ints("parents", parents, dev, (cache.sequences, T))
     if out is None:
-        out = torch.empty((rows, width), dtype=torch.bfloat16, device=dev)
+        out = q.new_empty((rows, width))
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (rows, width) or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out: contiguous bf16 {(rows, width)} on {dev} is expected")
     if prefix is not None and prefix.device != dev:
@@ -946,7 +946,6 @@ def stack_attn_decode_batch_workspace_bytes(cache: KVCache, prefix_len: int, tok
 def stack_kv_read(cache: KVCache, rows: int, starts=None, k=None, v=None, stream=None):
     """Cache rows starts[b] .. starts[b] + rows - 1 of every sequence (starts int32 [sequences]
     on the device; None: from row 0) as bf16 k, v [sequences, kv_heads, rows, head_dim]."""
-    import torch
     ctx = _elsewhere(cache.device, stream)
     if ctx is not None:
         with ctx:
@@ -954,15 +953,17 @@ def stack_kv_read(cache: KVCache, rows: int, starts=None, k=None, v=None, stream
     shape = (cache.sequences, cache.kv_heads, rows, cache.head_dim)
     if starts is not None:
         _ints("starts", starts, cache.device, (cache.sequences,))
-    k, v = (torch.empty(shape, dtype=torch.bfloat16, device=cache.device) if t is None else t for t in (k, v))
-    _cache_rows(k, v, shape, cache.device)
+    _cache_rows([t for t in (k, v) if t is not None], shape, cache.device)
+    bf16 = cache.k[0 if cache.bits == 16 else 1]
+    k = bf16.new_empty(shape) if k is None else k
+    v = bf16.new_empty(shape) if v is None else v
     check(lib.dflash_stack_kv_read(cache.ref, _ptr(starts), rows, _ptr(k), _ptr(v), _current_stream()))
     return k, v
 
 
-def _cache_rows(k, v, shape, device):
+def _cache_rows(tensors, shape, device):
     import torch
-    for t in (k, v):
+    for t in tensors:
         if t.dtype != torch.bfloat16 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
             raise ValueError(f"cache rows: contiguous bf16 {shape} on {device} are expected, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
@@ -975,7 +976,7 @@ def stack_kv_write(cache: KVCache, k, v, starts=None, stream=None):
     if ctx is not None:
         with ctx:
             return stack_kv_write(cache, k, v, starts)
-    _cache_rows(k, v, (cache.sequences, cache.kv_heads, k.shape[2], cache.head_dim), cache.device)
+    _cache_rows((k, v), (cache.sequences, cache.kv_heads, k.shape[2], cache.head_dim), cache.device)
     if starts is not None:
         _ints("starts", starts, cache.device, (cache.sequences,))
     check(lib.dflash_stack_kv_write(cache.ref, _ptr(starts), k.shape[2], _ptr(k), _ptr(v), _current_stream()))
@@ -1015,9 +1016,9 @@ def logprobs(logits, tokens=None, top: int = 0, stream=None) -> dict:
     if tokens is not None:
         n = tokens.shape[1] if tokens.dim() == 2 else -1
         _ints("tokens", tokens, dev, (rows, n))
-    f32 = dict(dtype=torch.float32, device=dev)
-    logp, entropy, best = (torch.empty(s, **f32) for s in ((rows, n), (rows,), (rows, top)))
-    ids = torch.empty((rows, top), dtype=torch.int32, device=dev)
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    logp, best = entropy.new_empty((rows, n)), entropy.new_empty((rows, top))
+    ids = torch.empty((rows, top), dtype=torch.int32, device=dev) if tokens is None else tokens.new_empty((rows, top))
     check(lib.dflash_logprobs(_ptr(logits), LOGITS_BF16 if logits.dtype == torch.bfloat16 else LOGITS_FP32,
                               logits.stride(0) if rows > 1 else vocab, rows, vocab, _ptr(tokens), n, top, _ptr(logp),
                               _ptr(entropy), _ptr(ids), _ptr(best), _current_stream()))
