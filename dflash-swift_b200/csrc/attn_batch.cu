@@ -27,13 +27,13 @@
 //
 // Measured in a captured graph, join included (256 dims, 24 q heads on 4 kv heads, groups of 64): a block of 8 tokens
 // over 1024 rows of 8 bits 17.5 us; over 131071 rows 103 us (2.8 TB/s; HBM alone would take 44); 33 sequences of one token
-// over about 4096 rows of 4 bits 92 us; 64 sequences of 4 tokens that share 32768 bf16 rows 448 us (0.46 PFLOP/s); with
+// over about 4096 rows of 4 bits 92 us; 64 sequences of 4 tokens that share 32768 bf16 rows 254 us (0.81 PFLOP/s); with
 // 128 dims, 16 q heads on 2 kv heads, 2 x 509 tokens over about 7000 rows of 8 bits 150 us.  Over quantised caches no
 // unit is full (131071 rows: instructions, mostly the unpack's and the softmax's, take 52 % of the issue slots, shared memory's
 // banks are 30 % busy, the tensor cores 17 %): the chain from codes to boxes to S to P to O, which two or three slots
-// overlap only in part, bounds it.  Over bf16 caches of 256 dims it is the ring, whose three slots leave a tile's
-// loads partly exposed (5 thousand cycles a tile against 2 of products).  Both have some 25 us beside their tiles:
-// launch, first loads, the change of units and the join (11 us there).
+// overlap only in part, bounds it.  Over bf16 caches the products take about half of a tile's time, the rest is the same
+// chain and the change of units.  Both have some 25 us beside their tiles: launch, first loads, the changes of units
+// (5 us each) and the join (11 us there).
 #include "common.cuh"
 #include "dflash_batch.h"
 #include "tcgen05.cuh"
@@ -56,6 +56,10 @@ constexpr int kMaxCtas = 160;              // partials are sized for this many C
 constexpr int kMaxSlots = 10;              // ring slots: two boxes each, one where d is 64
 constexpr int kMaxStages = 8;              // staging slots for codes: 64 or 128 rows each
 constexpr int kScaleDepth = 2;             // tiles whose key factors may be alive at once
+// Tiles that take as long as the change to another unit, about.  64 sequences of 200 rows behind a bf16 prefix of 32768: 451 us
+// with none, 287 with 1, 295 with 2, 254 with 4, 308 with 6; 32 of 250 rows behind 8190 of 8 bits: 47.3, 40.5, 41.0, 47.5 with
+// none, 1, 2 and 4 (long sequences: 92.7, 93.2, 92.1, 91.4).
+__host__ __device__ constexpr int unit_cost(int bits) { return bits == 16 ? 4 : 2; }
 constexpr int kPoison = 16;                // units whose poison flags may be alive at once
 constexpr float kLazy = 4.f;               // a maximum moves when a score passes it by 2^4 ...
 constexpr float kLift = 8.f;               // ... and P is 2^8 p, up to 2^12: small weights stay normal in fp16
@@ -76,9 +80,9 @@ struct Fixed {
     float part[4][kRows];
     float key_k[kScaleDepth][kKeys], key_v[kScaleDepth][kKeys];
     int poison[kPoison];
-    int abort, tmem, w0, w1, entry, off;
+    int abort, tmem, w0, w1, entry, off, pad;
     int unit_tiles, unit_rows;          // for the issuing thread, from the softmax warps
-    int warp_sum[kThreads / 32];
+    int warp_sum[2][kThreads / 32];
 };
 static_assert(offsetof(Fixed, base) % 16 == 0 && offsetof(Fixed, qs) % 16 == 0 &&
                   alignof(Fixed) == 16, "vector accesses");
@@ -166,9 +170,12 @@ __device__ __forceinline__ int entry_tiles(const Args& a, int e) {
     return len < 0 ? 0 : (own_keys(a, len, e - seq * a.blocks_o) + kKeys - 1) / kKeys;
 }
 
+// A run counts places: a tile of the prefix is one, and a (row block, kv head) of a sequence has `pad` of them before its
+// tiles', so that a run with many short units has fewer tiles.
 struct Walker {
-    int w, w1;          // next tile and end of the run
-    int entry, off;     // own region: current (sequence, row block) and its first tile
+    int w, w1;          // next place and end of the run
+    int entry, off;     // own region: current (sequence, row block) and its first place
+    int pad;
     __device__ __forceinline__ bool next(const Args& a, Unit& u) {
         if (w >= w1) return false;
         const int tiles_p = (a.prefix_len + kKeys - 1) / kKeys, prefix_end = tiles_p * a.blocks_p * a.cache.hkv;
@@ -183,26 +190,32 @@ struct Walker {
             u.t0 = w - s * tiles_p;
             u.rows = min(a.rb, a.cache.sequences * a.tokens * a.G - u.block * a.rb);
             u.len = u.keys = a.prefix_len;
+            u.n = min(tiles_p - u.t0, w1 - w);
+            w += u.n;
         } else {
-            int tiles = entry_tiles(a, entry);
-            while (w >= off + tiles * a.cache.hkv) {
-                off += tiles * a.cache.hkv;
+            int tiles = entry_tiles(a, entry), places = tiles ? tiles + pad : 0;
+            while (w >= off + places * a.cache.hkv) {
+                off += places * a.cache.hkv;
                 tiles = entry_tiles(a, ++entry);
+                places = tiles ? tiles + pad : 0;
             }
             const int rel = w - off;
             u.prefix = false;
-            u.head = rel / tiles;
+            u.head = rel / places;
             u.seq = a.blocks_o == 1 ? entry : entry / a.blocks_o;
             u.block = entry - u.seq * a.blocks_o;
             u.segment = (long long)entry * a.cache.hkv + u.head;
             u.tiles = tiles;
-            u.t0 = rel - u.head * tiles;
+            const int first = rel - u.head * places - pad;  // below 0: places without a tile
+            u.t0 = max(first, 0);
             u.rows = min(a.rb, a.tokens * a.G - u.block * a.rb);
             u.len = a.lengths[u.seq];
             u.keys = own_keys(a, u.len, u.block);
+            const int left = min(tiles - first, w1 - w);  // places of the run in here
+            w += left;
+            u.n = left + min(first, 0);
+            if (u.n <= 0) return false;  // the run ends before the first tile
         }
-        u.n = min(u.tiles - u.t0, w1 - w);
-        w += u.n;
         return true;
     }
 };
@@ -1008,28 +1021,43 @@ struct Kernel {
         const int per = (entries + kThreads - 1) / kThreads;
         const int e0 = min(entries, tid * per), e1 = min(entries, e0 + per);
         const int tiles_p = (a.prefix_len + kKeys - 1) / kKeys, prefix_end = tiles_p * a.blocks_p * a.cache.hkv;
-        int sum = 0;
+        int sum = 0, live = 0;
         for (int e = e0; e < e1; ++e) {
             if (e % a.blocks_o == 0 && blockIdx.x == 0) kv::block_start(a.lengths, e / a.blocks_o, a.tokens, a.cache.max_len);
-            sum += entry_tiles(a, e) * a.cache.hkv;
+            const int tiles = entry_tiles(a, e);
+            sum += tiles * a.cache.hkv;
+            live += tiles ? a.cache.hkv : 0;
         }
-        int* s_warp = fixed().warp_sum;
         const int warp = tid >> 5, lane = tid & 31;
-        int scan = sum;
+        int scan = sum, scan_live = live;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, scan, o);
-            if (lane >= o) scan += v;
+            const int v = __shfl_up_sync(0xffffffffu, scan, o), x = __shfl_up_sync(0xffffffffu, scan_live, o);
+            if (lane >= o) {
+                scan += v;
+                scan_live += x;
+            }
         }
-        if (lane == 31) s_warp[warp] = scan;
+        if (lane == 31) {
+            fixed().warp_sum[0][warp] = scan;
+            fixed().warp_sum[1][warp] = scan_live;
+        }
         __syncthreads();
-        int before = prefix_end + scan - sum, total = prefix_end;
+        int before = prefix_end + scan - sum, before_live = scan_live - live, total = prefix_end, all_live = 0;
         for (int i = 0; i < kThreads / 32; ++i) {
-            if (i < warp) before += s_warp[i];
-            total += s_warp[i];
+            if (i < warp) {
+                before += fixed().warp_sum[0][i];
+                before_live += fixed().warp_sum[1][i];
+            }
+            total += fixed().warp_sum[0][i];
+            all_live += fixed().warp_sum[1][i];
         }
+        // no places without tiles where each CTA has one tile at most: they would put two into some
+        const int pad = total > static_cast<int>(gridDim.x) ? unit_cost(BITS) : 0;
+        sum += live * pad;
+        before += before_live * pad;
         // with nothing but absent sequences the prefix has no reader
-        if (total == prefix_end) total = 0;
+        total = all_live ? total + all_live * pad : 0;
         const int ctas = min(static_cast<int>(gridDim.x), total), cta = blockIdx.x;
         const auto share = [&](int c) {  // floor(total c / ctas)
             return total < (1 << 23) ? static_cast<int>(static_cast<uint32_t>(total * c) / static_cast<uint32_t>(ctas))
@@ -1041,13 +1069,18 @@ struct Kernel {
             fixed().w0 = w0;
             fixed().w1 = w1;
             fixed().entry = fixed().off = 0;
+            fixed().pad = pad;
         }
         __syncthreads();
         if (w < w1 && before <= w && w < before + sum) {
-            int off = before, e = e0, n = entry_tiles(a, e) * a.cache.hkv;
+            const auto places = [&](int x) {
+                const int tiles = entry_tiles(a, x);
+                return tiles ? (tiles + pad) * a.cache.hkv : 0;
+            };
+            int off = before, e = e0, n = places(e);
             while (w >= off + n) {
                 off += n;
-                n = entry_tiles(a, ++e) * a.cache.hkv;
+                n = places(++e);
             }
             fixed().entry = e;
             fixed().off = off;
@@ -1090,7 +1123,7 @@ struct Kernel {
         __syncthreads();
         tc5::fence_after();
         const uint32_t tmem = *reinterpret_cast<volatile int*>(&fixed().tmem);
-        const Walker w{fixed().w0, fixed().w1, fixed().entry, fixed().off};
+        const Walker w{fixed().w0, fixed().w1, fixed().entry, fixed().off, fixed().pad};
         if (warp < kSoftmaxWarps) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             softmax(a, w, tmem, blockIdx.x);
@@ -1268,7 +1301,7 @@ static int check(const dflash_kv_cache* cache, const dflash_kv_cache* prefix, in
     if (G > 64 || (long long)cache->sequences * tokens > 0x7fffffffll / hq ||
         (long long)prefix_len + cache->max_len > 0x7fffffffll - kKeys ||
         blocks_p * cache->kv_heads * ((prefix_len + kKeys - 1ll) / kKeys) +
-                cache->sequences * blocks_o * cache->kv_heads * tiles > 0x7fffffffll)
+                cache->sequences * blocks_o * cache->kv_heads * (tiles + unit_cost(cache->bits)) > 0x7fffffffll)
         return fail(DFLASH_ERR_UNSUPPORTED, "%s: too many rows or keys, or more than 64 q heads per kv head", who);
     if (prefix_len > 0 && prefix) {
         const int sp = kv::check_cache(prefix, who);
