@@ -62,9 +62,9 @@ __device__ __forceinline__ float ex2(float x) {
 struct Sums {
     float m, l, w;
     __device__ __forceinline__ void raise(float to) {  // m becomes the larger `to`
-        const float d = (m - to) * kLog2e;             // -inf only where l is 0
+        const float d = (m - to) * kLog2e;             // may be -inf, as may l d: far below `to`, or nothing yet
         const float f = ex2(d);
-        w = l == 0.f ? 0.f : f * fmaf(l, d, w);
+        w = f == 0.f ? 0.f : f * fmaf(l, d, w);        // a weight of 0 takes no part (0 x inf would be NaN)
         l *= f;
         m = to;
     }
