@@ -120,34 +120,59 @@ __device__ __forceinline__ void load_floats(const float* p, float (&x)[CH]) {
 // the even z on every path.  s and b are rounded to bf16, their stored form, BEFORE the codes
 // are taken from them: with codes from the unrounded scale the 2^-9 of the scale would cost up
 // to half a step at code 255.  Where (max - min) / L is under 1e-7 the step is 1e-7.
+// A group with an element of kLargest or more, whose e L or max - min could pass fp32's range, is taken down
+// by 2^-64 first and its scale and bias up again: powers of two, which change no rounding.
+constexpr float kLargest = 6.6461399789245794e35f;  // 2^119
+
 template <int CH>
-__device__ __forceinline__ void quantise_row(const float (&x)[CH], int lane, int bits, int group, uint8_t* codes,
+__device__ __forceinline__ void quantise_row(float (&x)[CH], int lane, int bits, int group, uint8_t* codes,
                                              uint16_t* scales, uint16_t* biases) {
     const float top = bits == 8 ? 255.f : 15.f;
     const int width = group / CH;  // lanes of a group, a power of two
     float lo = x[0], hi = x[0];
-    bool finite = true;
+    bool small = true;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         lo = fminf(lo, x[i]);
         hi = fmaxf(hi, x[i]);
-        finite = finite && fabsf(x[i]) < INFINITY;
+        small = small && fabsf(x[i]) < kLargest;
     }
+    const uint32_t large = __ballot_sync(0xffffffffu, !small);
     for (int o = 1; o < width; o <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     const uint32_t members = (width == 32 ? 0xffffffffu : (1u << width) - 1u) << (lane & ~(width - 1));
-    const bool bad = (__ballot_sync(0xffffffffu, !finite) & members) != 0;
+    bool bad = false;
+    float up = 1.f, least = 1e-7f;
+    if (large) {  // of the row, so seldom
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) finite = finite && fabsf(x[i]) < INFINITY;
+        bad = (__ballot_sync(0xffffffffu, !finite) & members) != 0;
+        if (large & members) {
+            const float down = 5.421010862427522e-20f;  // 2^-64
+            up = 18446744073709551616.f;
+            least *= down;
+            lo *= down;
+            hi *= down;
+#pragma unroll
+            for (int i = 0; i < CH; ++i) x[i] *= down;
+        }
+    }
     const bool low = fabsf(lo) > fabsf(hi);
     const float edge = low ? lo : hi, sign = low ? 1.f : -1.f, span = hi - lo;
-    const bool tiny = span / top < 1e-7f;
-    const float z = sign * rintf(tiny ? edge / 1e-7f : edge * top / span);
-    float s = z != 0.f ? edge / z : sign * fmaxf(span / top, 1e-7f);
+    const bool tiny = span / top < least;
+    const float z = sign * rintf(tiny ? edge / least : edge * top / span);
+    float s = z != 0.f ? edge / z : sign * fmaxf(span / top, least);
     float b = z != 0.f ? edge : 0.f;
     if (bad) s = b = __int_as_float(0x7fc00000);
-    const uint16_t sb = bf_bits(s), bb = bf_bits(b);
+    uint16_t sb = bf_bits(s), bb = bf_bits(b);
     const float sr = __uint_as_float(static_cast<uint32_t>(sb) << 16), br = __uint_as_float(static_cast<uint32_t>(bb) << 16);
+    if (large) {
+        sb = bf_bits(sr * up);
+        bb = bf_bits(br * up);
+    }
     if ((lane & (width - 1)) == 0) {
         scales[lane / width] = sb;
         biases[lane / width] = bb;
@@ -192,7 +217,7 @@ __device__ __forceinline__ void quantise_row(const float (&x)[CH], int lane, int
 
 // Writes one row that a warp holds to the cache in its format.
 template <int CH>
-__device__ __forceinline__ void store_cache_row(const View& cache, bool is_v, int64_t cr, int lane, const float (&x)[CH]) {
+__device__ __forceinline__ void store_cache_row(const View& cache, bool is_v, int64_t cr, int lane, float (&x)[CH]) {
     constexpr int d = CH * 32;
     uint8_t* base = (is_v ? cache.v : cache.k) + cr * (d * cache.bits / 8);
     if (cache.bits == 16) {

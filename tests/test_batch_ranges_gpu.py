@@ -4,7 +4,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_batch_gpu import gen, logprob_want, near
+import batch_ref as R
+from test_batch_gpu import gen, lens_tensor, logprob_want, near
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +32,25 @@ def test_rows_masked_by_a_large_negative_number(dc, cuda, dtype, R_, V, mask):
     assert torch.equal(got["top_ids"].long(), ids)
     assert near(got["logprobs"], given) and near(got["top_logprobs"], best)
     assert near(got["entropy"], ent, 2.0 ** -16 * (lp.exp() * lp).abs().sum(-1))
+
+
+# ----------------------------------------------------------------------------- quantisation
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("kind", ["normal", "signs", "constant", "wide", "one"])
+def test_groups_of_the_largest_numbers(dc, cuda, bits, kind):
+    """Finite groups whose edge times 2^bits - 1, or whose range, passes fp32's."""
+    x = torch.rand(1, 2, 6, 128, generator=gen(105, cuda), device=cuda)
+    x = {"normal": 1e37 * torch.randn(x.shape, generator=gen(106, cuda), device=cuda), "signs": torch.sign(x - 0.5) * 2e38,
+         "constant": 0 * x - 3e38, "wide": x * 3.3e38 - (x > 0.5) * 3.3e38, "one": x}[kind]
+    if kind == "one":  # one group of a row, beside ordinary ones
+        x[0, 0, :, 64:] *= 2e37
+    x = x.to(torch.bfloat16)
+    assert x.isfinite().all()
+    cache = dc.KVCache(1, 2, 8, 128, bits, 32, cuda)
+    dc.stack_kv_write(cache, x, x, starts=lens_tensor([1], cuda))
+    k, v = dc.stack_kv_read(cache, 6, starts=lens_tensor([1], cuda))
+    torch.cuda.synchronize()
+    assert dc.device_error() == 0 and torch.equal(k, v)
+    want = R.values(R.quantise(x.double(), bits, 32), bits, 32)
+    assert torch.equal(k.double(), want.to(torch.bfloat16).double())
