@@ -293,6 +293,9 @@ __device__ __forceinline__ bool bar_any(int id, int threads, bool v) {
     return r != 0;
 }
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }  // 2^e, e in -126 .. 127
+__device__ __forceinline__ float exp2_any(int e) {  // 2^e, e in -149 .. 127
+    return e < -126 ? __int_as_float(1 << (e + 149)) : exp2i(e);
+}
 // Exponent of |a| for the scaling: 0 for zero, infinity and NaN.
 __device__ __forceinline__ int exponent(float a) {
     const int e = (__float_as_int(a) >> 23) & 255;
@@ -310,7 +313,8 @@ template <int BITS, int D>
 struct Kernel {
     static constexpr bool kQuant = BITS != 16;
     // Keys are scaled to 2^kTop .. 2^(kTop + 1): the step of a group, at most 2^(kTop + 2) / (2^BITS - 1), has
-    // to stay under 2^-8 (store_groups).
+    // to stay under 2^-8 (store_groups).  An element under 2^(-14 - kTop) of its key's largest is subnormal in fp16 and
+    // held to 2^(-25 - kTop) of that.
     static constexpr int kTop = BITS == 8 ? -3 : -7;
     // 16 softmax warps, four per TMEM lane quarter with 32 columns each, and 8 producers; over quantised caches of 256
     // dims, whose row blocks have 64 rows (all their columns belong to eight warps) and whose codes take twice the
@@ -522,14 +526,14 @@ struct Kernel {
                 }
         }
     }
-    // Largest magnitude that a lane's groups can stand for.
+    // A quarter of the largest magnitude that a lane's groups can stand for (the whole could pass fp32's range by a rounding).
     __device__ static __forceinline__ float largest(const Groups& g) {
-        constexpr float kCodes = BITS == 8 ? 255.f : 15.f;
+        constexpr float kCodes = BITS == 8 ? 63.75f : 3.75f;
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {  // zero where there is none
             const float s0 = __uint_as_float(g.s[i] << 16), s1 = __uint_as_float(g.s[i] & 0xffff0000u);
-            const float b0 = __uint_as_float(g.b[i] << 16), b1 = __uint_as_float(g.b[i] & 0xffff0000u);
+            const float b0 = 0.25f * __uint_as_float(g.b[i] << 16), b1 = 0.25f * __uint_as_float(g.b[i] & 0xffff0000u);
             m = largest_of(m, b0, fmaf(kCodes, s0, b0));
             m = largest_of(m, b1, fmaf(kCodes, s1, b1));
         }
@@ -667,14 +671,15 @@ struct Kernel {
                         const float other = __shfl_xor_sync(0xffffffffu, top, 16);
                         asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(other));
                     }
-                    const int e = min(max(exponent(top), -100), 100);
+                    // every finite size up to the largest: 2^(kTop - e) may be subnormal, which a product takes as it is
+                    const int e = top > 0.f && top < INFINITY ? min(max(exponent(top) + 2, -100), 127) : 0;
                     store_groups(tables + (is_v ? (tile & 1) * table_bytes : 0) + key_of * groups * 4, g, groups, first,
-                                 exp2i(kTop - e));
+                                 exp2_any(kTop - e));
                     if (lane < kOwn) {
                         if (is_v) {
                             fixed().key_v[depth][key_of] = e;
                         } else {
-                            fixed().key_k[depth][key_of] = exp2i(e - kTop);
+                            fixed().key_k[depth][key_of] = exp2i(e - kTop - kTopQ);
                         }
                     }
                     bad = __any_sync(0xffffffffu, !(top < INFINITY));
@@ -797,12 +802,12 @@ struct Kernel {
                     }
 #pragma unroll
                     for (int o = 1; o < kPer; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    const int e = min(max(exponent(m), -100), 120);
+                    const int e = max(exponent(m), kTopQ - 126);
                     const float sc = exp2i(kTopQ - e);
                     uint32_t* p = &y.x;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) p[i] = pack2<false>(f[order<BITS>(2 * i)] * sc, f[order<BITS>(2 * i + 1)] * sc);
-                    if (c == 0 && n < u.rows) fixed().qs[n] = a.scale * 1.4426950408889634f * exp2i(e - kTopQ);
+                    if (c == 0 && n < u.rows) fixed().qs[n] = a.scale * 1.4426950408889634f * exp2i(e);
                 }
                 if (n < u.rows) sts128(smem_at(a.l.q) + (c >> 3) * a.nr * 128 + n * 128 + (((c & 7) ^ (n & 7)) << 4), y);
             }
@@ -855,7 +860,7 @@ struct Kernel {
                 const int at = (u.t0 + i) * kKeys;
                 const int b = at + key - u.len;  // block row of the key; a prefix ends where its block would begin
                 const bool masked = at + kKeys > u.len;
-                const float weight = kQuant ? exp2i(-static_cast<int>(ev)) : 1.f;
+                const float weight = kQuant ? exp2_any(-static_cast<int>(ev)) : 1.f;
                 bool waited = i == 0;  // for the last tile's p V: P and the accumulators are free
                 const auto hand_over = [&]() {
                     fence_proxy_async_shared();
@@ -874,11 +879,11 @@ struct Kernel {
                             float4 bs = *reinterpret_cast<const float4*>(&fixed().base[n0 + j]);
                             if (raise) bs = make_float4(0.f, 0.f, 0.f, 0.f);
                             if (kQuant) {
-                                const float4 qs = *reinterpret_cast<const float4*>(&fixed().qs[n0 + j]);
+                                float4 qs = *reinterpret_cast<const float4*>(&fixed().qs[n0 + j]);
                                 add2(bs.x, bs.y, ev, ev);
                                 add2(bs.z, bs.w, ev, ev);
-                                mul2(y[j], y[j + 1], ks, ks);
-                                mul2(y[j + 2], y[j + 3], ks, ks);
+                                mul2(qs.x, qs.y, ks, ks);  // the factors first: each with y alone could pass fp32's range
+                                mul2(qs.z, qs.w, ks, ks);
                                 fma2(y[j], y[j + 1], qs.x, qs.y, bs.x, bs.y);
                                 fma2(y[j + 2], y[j + 3], qs.z, qs.w, bs.z, bs.w);
                             } else {

@@ -1,11 +1,12 @@
-"""The batch entries at the ends of their types' ranges, against 64-bit statements."""
+"""The batch entries at the ends of their types' ranges, against the 64-bit statements of batch_ref:
+logits masked by large negative numbers, cached rows of any finite size."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 import batch_ref as R
-from test_batch_gpu import gen, lens_tensor, logprob_want, near
+from test_batch_gpu import attention_case, attention_want, check_rows, gen, lens_tensor, logprob_want, near
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +55,75 @@ def test_groups_of_the_largest_numbers(dc, cuda, bits, kind):
     assert dc.device_error() == 0 and torch.equal(k, v)
     want = R.values(R.quantise(x.double(), bits, 32), bits, 32)
     assert torch.equal(k.double(), want.to(torch.bfloat16).double())
+
+
+# ----------------------------------------------------------------------------- attention
+
+def stored(size, shape, bits, group, seed, dev):
+    """Cache rows whose values are about `size` (a number, or one per row): random codes, scales and
+    biases, not held to the smallest step that the write rule keeps."""
+    g = gen(seed, dev)
+    *lead, d = shape
+    size = torch.as_tensor(size, dtype=torch.float64, device=dev)
+    words = torch.randint(-2 ** 31, 2 ** 31, (*lead, d * bits // 32), generator=g, device=dev).to(torch.int32)
+    r = lambda: torch.rand(*lead, d // group, generator=g, device=dev).double()  # noqa: E731
+    scale = (0.5 + r()) * size / (2 ** bits - 1)
+    return words, scale.to(torch.bfloat16), (-(0.25 + 0.5 * r()) * size).to(torch.bfloat16)
+
+
+def put(part, new):
+    for t, n in zip(part, new):
+        if t is not None:
+            t.copy_(n)
+
+
+QUANT = [(8, 64, 128), (4, 32, 128), (8, 128, 256), (4, 64, 64)]
+
+
+@pytest.mark.parametrize("bits,group,d", QUANT)
+@pytest.mark.parametrize("size", [1e29, 1e32, 1e35, 1e37])
+@pytest.mark.parametrize("tree", [False, True])
+def test_finite_rows_of_any_size_that_a_token_does_not_see(dc, cuda, bits, group, d, size, tree):
+    """The last block rows' k and v, finite but large, reach the tokens that see them alone."""
+    case = (2, 6, 8, 2, d, bits, group, [125, 30], 20)
+    S, T = case[:2]
+    q, gate, cache, prefix, _ = attention_case(dc, cuda, case, seed=111)
+    parents = torch.tensor([[-1, 0, 0, 1, 2, 2]] * 2, dtype=torch.int32) if tree else None
+    want, tol = attention_want(q, gate, cache, prefix, parents, case, d ** -0.5)
+    for b, n in enumerate(case[7]):
+        for part, s in ((cache.k, 1), (cache.v, 2)):
+            big = stored(size, (2, 1, d), bits, group, 113 + s, cuda)
+            for t, x in zip(part, big):
+                t[b, :, n + T - 1:n + T] = x
+    out = dc.stack_attn_decode_batch(q, cache, lens_tensor(case[7], cuda), d ** -0.5, gate=gate, prefix=prefix,
+                                     prefix_len=20, parents=None if parents is None else parents.to(cuda))
+    torch.cuda.synchronize()
+    assert dc.device_error() == 0
+    good = torch.ones(S * T, dtype=torch.bool, device=cuda)
+    good[[T - 1, 2 * T - 1]] = False
+    check_rows(out[good], want[good], tol[good])
+
+
+@pytest.mark.parametrize("bits,group,d", QUANT)
+@pytest.mark.parametrize("size", [1e-25, 1e-15, 1e15, 1e29, 1e32, 1e35, 1e37])
+def test_values_of_any_finite_size(dc, cuda, bits, group, d, size):
+    case = (2, 3, 4, 2, d, bits, group, [40, 300], 130)
+    q, gate, cache, prefix, _ = attention_case(dc, cuda, case, seed=121)
+    for c, s in ((cache, 5), (prefix, 6)):
+        put(c.v, stored(size, (c.sequences, 2, c.max_len, d), bits, group, s, cuda))
+    out = dc.stack_attn_decode_batch(q, cache, lens_tensor(case[7], cuda), d ** -0.5, prefix=prefix, prefix_len=130)
+    want, tol = attention_want(q, None, cache, prefix, None, case, d ** -0.5)
+    check_rows(out, want, tol)
+
+
+@pytest.mark.parametrize("bits,group,d", QUANT)
+@pytest.mark.parametrize("size,q_size", [(1e32, 1e-31), (1e36, 3e-35), (1e-25, 1e25), (1e-30, 1e33)])
+def test_keys_and_queries_of_any_finite_size(dc, cuda, bits, group, d, size, q_size):
+    case = (2, 3, 4, 2, d, bits, group, [40, 300], 130)
+    q, gate, cache, prefix, _ = attention_case(dc, cuda, case, seed=131, q_std=q_size)
+    for c, s in ((cache, 7), (prefix, 8)):
+        put(c.k, stored(size, (c.sequences, 2, c.max_len, d), bits, group, s, cuda))
+    scale = d ** -0.5 / (size * q_size)
+    out = dc.stack_attn_decode_batch(q, cache, lens_tensor(case[7], cuda), scale, prefix=prefix, prefix_len=130)
+    want, tol = attention_want(q, None, cache, prefix, None, case, scale)
+    check_rows(out, want, tol)
