@@ -64,6 +64,10 @@ constexpr int kPoison = 16;                // units whose poison flags may be al
 constexpr float kLazy = 4.f;               // a maximum moves when a score passes it by 2^4 ...
 constexpr float kLift = 8.f;               // ... and P is 2^8 p, up to 2^12: small weights stay normal in fp16
 constexpr float kNever = 3e38f;            // base of a row without a maximum yet: every score passes it
+// A key's factor 2^e goes into its P and out of its sum's weight, so P of two keys may be 2^(e - e') apart at the same score:
+// exact sums as long as the values' sizes differ by no more than 2^126, which ex2 and the join's weights reach.
+constexpr int kZero = -62;                 // exponent of a row of zeros: halfway, so beside sizes of 2^-84 to 2^64
+constexpr float kTiny = 2.350988701644575e-38f;  // 2^-125: smaller rows (top is a quarter) count as zeros
 constexpr int kTopQ = 12;                  // query rows are scaled to 2^12 .. 2^13 in fp16
 constexpr uint32_t kTmemColumns = 512;
 constexpr int kAllSoftmax = 5;               // named barrier of all softmax warps; 1 to 4: of those with the same columns
@@ -671,8 +675,11 @@ struct Kernel {
                         const float other = __shfl_xor_sync(0xffffffffu, top, 16);
                         asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(other));
                     }
-                    // every finite size up to the largest: 2^(kTop - e) may be subnormal, which a product takes as it is
-                    const int e = top > 0.f && top < INFINITY ? min(max(exponent(top) + 2, -100), 127) : 0;
+                    // Every finite size up to the largest: 2^(kTop - e) may be subnormal, which a product takes as it is.
+                    // A row of zeros, whose exponent could be any, counts as smaller than what it lies beside (V's goes
+                    // into the maxima, and must not hold those of small rows up), but no smaller than kZero: its
+                    // weight is the softmax's still.
+                    const int e = !(top < INFINITY) ? 0 : top < kTiny ? kZero : min(max(exponent(top) + 2, -100), 127);
                     store_groups(tables + (is_v ? (tile & 1) * table_bytes : 0) + key_of * groups * 4, g, groups, first,
                                  exp2_any(kTop - e));
                     if (lane < kOwn) {

@@ -1,5 +1,5 @@
 """The batch entries at the ends of their types' ranges, against the 64-bit statements of batch_ref:
-logits masked by large negative numbers, cached rows of any finite size."""
+logits masked by large negative numbers, cached rows of any finite size, rows of zeros."""
 from __future__ import annotations
 
 import pytest
@@ -126,4 +126,33 @@ def test_keys_and_queries_of_any_finite_size(dc, cuda, bits, group, d, size, q_s
     scale = d ** -0.5 / (size * q_size)
     out = dc.stack_attn_decode_batch(q, cache, lens_tensor(case[7], cuda), scale, prefix=prefix, prefix_len=130)
     want, tol = attention_want(q, None, cache, prefix, None, case, scale)
+    check_rows(out, want, tol)
+
+
+@pytest.mark.parametrize("bits,group,d", QUANT)
+@pytest.mark.parametrize("size", [1e-20, 1e-12, 1e-10, 1e-8, 1.0, 1e15])
+def test_values_beside_rows_of_zeros(dc, cuda, bits, group, d, size):
+    """Rows whose codes, scales and biases are all zero take their share of the weight, and the others keep their bits."""
+    case = (2, 3, 4, 2, d, bits, group, [40, 300], 130)
+    q, gate, cache, prefix, _ = attention_case(dc, cuda, case, seed=141)
+    for c, s in ((cache, 9), (prefix, 10)):
+        put(c.v, stored(size, (c.sequences, 2, c.max_len, d), bits, group, s, cuda))
+        for t in c.v:
+            t[:, :, ::3] = 0
+    out = dc.stack_attn_decode_batch(q, cache, lens_tensor(case[7], cuda), d ** -0.5, prefix=prefix, prefix_len=130)
+    want, tol = attention_want(q, None, cache, prefix, None, case, d ** -0.5)
+    check_rows(out, want, tol)
+
+
+@pytest.mark.parametrize("bits,group,d", QUANT)
+@pytest.mark.parametrize("small,large", [(1e-10, 1e10), (1e-20, 1e12), (1.0, 1e30)])
+def test_values_of_very_different_sizes(dc, cuda, bits, group, d, small, large):
+    """Every other row is large: the small ones count in the denominator alone, in full."""
+    case = (2, 3, 4, 2, d, bits, group, [40, 300], 130)
+    q, gate, cache, prefix, _ = attention_case(dc, cuda, case, seed=151)
+    for c, s in ((cache, 11), (prefix, 12)):
+        size = torch.tensor([small, large], dtype=torch.float64).repeat((c.max_len + 1) // 2)[:c.max_len, None]
+        put(c.v, stored(size, (c.sequences, 2, c.max_len, d), bits, group, s, cuda))
+    out = dc.stack_attn_decode_batch(q, cache, lens_tensor(case[7], cuda), d ** -0.5, prefix=prefix, prefix_len=130)
+    want, tol = attention_want(q, None, cache, prefix, None, case, d ** -0.5)
     check_rows(out, want, tol)
