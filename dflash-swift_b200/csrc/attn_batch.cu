@@ -62,7 +62,6 @@ constexpr int kScaleDepth = 2;             // tiles whose key factors may be ali
 __host__ __device__ constexpr int unit_cost(int bits) { return bits == 16 ? 4 : 2; }
 constexpr int kPoison = 16;                // units whose poison flags may be alive at once
 constexpr float kLazy = 4.f;               // a maximum moves when a score passes it by 2^4 ...
-constexpr float kLift = 8.f;               // ... and P is 2^8 p, up to 2^12: small weights stay normal in fp16
 constexpr float kNever = 3e38f;            // base of a row without a maximum yet: every score passes it
 // A key's factor 2^e goes into its P and out of its sum's weight, so P of two keys may be 2^(e - e') apart at the same score:
 // exact sums as long as the values' sizes differ by no more than 2^126, which ex2 and the join's weights reach.
@@ -320,6 +319,9 @@ struct Kernel {
     // to stay under 2^-8 (store_groups).  An element under 2^(-14 - kTop) of its key's largest is subnormal in fp16 and
     // held to 2^(-25 - kTop) of that.
     static constexpr int kTop = BITS == 8 ? -3 : -7;
+    // P is 2^kLift p, and up to 2^kLazy more: in fp16 2^8, so that small weights stay normal; in bf16, which has fp32's range,
+    // 2^-16, so that the sum of p V over 2^12 keys stays in range for values up to the largest.
+    static constexpr float kLift = kQuant ? 8.f : -16.f;
     // 16 softmax warps, four per TMEM lane quarter with 32 columns each, and 8 producers; over quantised caches of 256
     // dims, whose row blocks have 64 rows (all their columns belong to eight warps) and whose codes take twice the
     // unpacking, 8 and 16.  (1018 tokens over 7000 rows of 8 bits and 128 dims: 150 us with sixteen, 175 with eight.)

@@ -156,3 +156,16 @@ def test_values_of_very_different_sizes(dc, cuda, bits, group, d, small, large):
     out = dc.stack_attn_decode_batch(q, cache, lens_tensor(case[7], cuda), d ** -0.5, prefix=prefix, prefix_len=130)
     want, tol = attention_want(q, None, cache, prefix, None, case, d ** -0.5)
     check_rows(out, want, tol)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("size", [1e-30, 1e-20, 1e33, 1e35, 1e36, 1e37])
+def test_bf16_values_of_any_size(dc, cuda, d, size):
+    """The sum of p V before its division stays in range wherever the plain sum of exp(s - max) V does."""
+    case = (2, 3, 4, 2, d, 16, 0, [40, 300], 130)
+    q, gate, cache, prefix, _ = attention_case(dc, cuda, case, seed=161)
+    for c, s in ((cache, 13), (prefix, 14)):
+        c.v[0].copy_(size * (torch.rand(c.v[0].shape, generator=gen(s, cuda), device=cuda) - 0.5))
+    out = dc.stack_attn_decode_batch(q, cache, lens_tensor(case[7], cuda), d ** -0.5, prefix=prefix, prefix_len=130)
+    want, tol = attention_want(q, None, cache, prefix, None, case, d ** -0.5)
+    check_rows(out, want, tol)
