@@ -692,6 +692,7 @@ struct Kernel {
                         }
                     }
                     bad = __any_sync(0xffffffffu, !(top < INFINITY));
+                    __syncwarp();  // the lanes' tables and factors, for the others and through lane 0's arrival (a vote orders nothing)
                     if (lane == 0) mbar_arrive(&fixed().sc_full[depth]);
                     if (i + 1 < cur.n) load_groups(a, cur, is_v, (cur.t0 + i + 1) * kKeys + key_of, groups, first, g);
                     else if (more) load_groups(a, next, is_v, next.t0 * kKeys + key_of, groups, first, g);
