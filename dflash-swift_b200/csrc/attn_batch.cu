@@ -76,7 +76,7 @@ constexpr int kSmemLimit = 232448;
 // tables, and from the next 1024-byte border on the ring, Q and P.
 struct Fixed {
     uint64_t full[kMaxSlots], empty[kMaxSlots], s_full[2], p_full, pv_done, q_full, sc_full[kScaleDepth],
-        sc_empty[kScaleDepth], staged[kMaxStages], unstaged[kMaxStages];
+        sc_empty[kScaleDepth], staged[kMaxStages], unstaged[kMaxStages], drained;
     alignas(16) float base[kRows];      // -(maximum - kLift): scores are taken relative to it; read four at a time, like qs
     float qs[kRows], corr[kRows], m[kRows];
     int info[kRows];                    // chain: the row's token; tree: its path mask
@@ -344,15 +344,22 @@ struct Kernel {
     // A bounded wait that stays small where it is inlined: a failed try sleeps for as long as the hardware
     // lets it (the phase's end wakes it), and 2^22 of them raise the error.  No clock is read, whose read
     // costs more than the usual wait.  After an error every wait returns at once and the roles run on to
-    // their ends.
+    // their ends; copies and products in flight are drained there, since the block's shared and tensor memory
+    // must not go, to another block perhaps, before them (0.2 us a call: the drains themselves find nothing to wait for).
+    __device__ static __forceinline__ bool aborted() { return *const_cast<volatile int*>(&fixed().abort) != 0; }
+    __device__ static __forceinline__ void give_up() {
+        atomicOr(&g_device_error, DFLASH_DEVERR_ATTN_PIPELINE);
+        *const_cast<volatile int*>(&fixed().abort) = 1;
+    }
     __device__ static __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
         if (mbar_try_wait(bar, parity)) return;
         for (int n = 0; !mbar_try_wait(bar, parity); ++n) {
-            if (*const_cast<volatile int*>(&fixed().abort)) return;
-            if (n == 1 << 22) {
-                atomicOr(&g_device_error, DFLASH_DEVERR_ATTN_PIPELINE);
-                *const_cast<volatile int*>(&fixed().abort) = 1;
-            }
+            if (aborted()) return;
+            if (n == 1 << 22) give_up();
+        }
+    }
+    __device__ static __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+        for (int n = 0; n < 1 << 22 && !mbar_try_wait(bar, parity); ++n) {
         }
     }
 
@@ -491,7 +498,14 @@ struct Kernel {
             const uint8_t* rows = is_v ? src.v : src.k;
 #pragma unroll 1
             for (int at = src.t0 * kKeys; at < (src.t0 + src.n) * kKeys; at += a.stage_rows) {
-                wait(&fixed().unstaged[slot], phase ^ 1);
+                // as wait(), but no copy goes to a slot that was not handed back
+                bool mine = mbar_try_wait(&fixed().unstaged[slot], phase ^ 1);
+#pragma unroll 1
+                for (int n = 0; !mine; ++n) {
+                    if (aborted()) goto out;
+                    if (n == 1 << 22) give_up();
+                    mine = mbar_try_wait(&fixed().unstaged[slot], phase ^ 1);
+                }
                 const uint32_t bytes = min(a.stage_rows, max(0, src.keys - at)) * (D * BITS / 8);
                 mbar_arrive_expect_tx(&fixed().staged[slot], bytes);
                 if (bytes)
@@ -503,6 +517,9 @@ struct Kernel {
                 }
             }
         }
+out:
+#pragma unroll 1
+        for (int i = first; i < first + a.stages; ++i) drain(&fixed().staged[i], i < slot ? phase : phase ^ 1);
     }
 
     // Scales and biases of one key, as raw bf16 pairs: up to two words of each, of four where a key has
@@ -1118,6 +1135,7 @@ struct Kernel {
             mbar_init(&fixed().p_full, kSubs);
             mbar_init(&fixed().pv_done, 1);
             mbar_init(&fixed().q_full, 1);
+            mbar_init(&fixed().drained, 1);
             for (int i = 0; i < kScaleDepth; ++i) {
                 mbar_init(&fixed().sc_full[i], kProducerWarps);
                 mbar_init(&fixed().sc_empty[i], kSoftmaxWarps);
@@ -1126,7 +1144,7 @@ struct Kernel {
                 mbar_init(&fixed().staged[i], 1);
                 mbar_init(&fixed().unstaged[i], kGroupWarps);
             }
-            fixed().abort = 0;
+            fixed().abort = fixed().unit_tiles = 0;
             fence_barrier_init();
         }
         if (threadIdx.x < kPoison) fixed().poison[threadIdx.x] = 0;
@@ -1155,7 +1173,13 @@ struct Kernel {
         }
         tc5::fence_before();
         __syncthreads();
-        if (warp == kIssueWarp) tc5::dealloc(tmem, kTmemColumns);
+        if (warp == kIssueWarp) {
+            if (aborted()) {  // else the softmax has waited for every product
+                if (tc5::elect()) tc5::commit(&fixed().drained);
+                drain(&fixed().drained, 0);
+            }
+            tc5::dealloc(tmem, kTmemColumns);
+        }
     }
 };
 
