@@ -821,6 +821,8 @@ def _elsewhere(device, stream):
     if device.type != "cuda":
         raise ValueError(f"tensors on {device}: the library runs on CUDA devices only")
     if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"a stream of {stream.device} for tensors on {device}")
         return torch.cuda.stream(stream)
     if device.index != torch.cuda.current_device():
         return torch.cuda.device(device)

@@ -3,6 +3,7 @@ before any CUDA call, and the binding refuses tensors that do not fit.  No GPU n
 from __future__ import annotations
 
 import ctypes
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -128,3 +129,10 @@ def test_the_binding_refuses_tensors_that_do_not_fit(dc):
         dc.logprobs(torch.zeros(2, 8))
     with pytest.raises(ValueError, match="CUDA"):
         dc.stack_attn_decode_batch(torch.zeros(1, 128, **bf), cache, torch.zeros(1, dtype=torch.int32), 0.1)
+
+
+def test_the_binding_refuses_a_stream_of_another_device(dc):
+    """Such a call would run on the tensors' device's current stream instead."""
+    stream = SimpleNamespace(device=torch.device("cuda", 1))
+    with pytest.raises(ValueError, match="stream"):
+        dc._elsewhere(torch.device("cuda", 0), stream)
