@@ -235,8 +235,9 @@ __device__ __forceinline__ void store_cache_row(const View& cache, bool is_v, in
 // the quantisation is a run of lanes.  Rotary: element i < rot / 2 pairs with i + rot / 2, which a whole
 // number of lanes further on holds (rot / 2 is a multiple of 32); the rows' cosines and sines are made
 // once per CTA and shared by its heads.  The angle is kept as a fraction of a turn in 64-bit fixed point:
-// position times the frequency's fraction wraps as the angle does, so far positions lose nothing (a
-// float product is off by 2^-24 of the angle, 0.06 rad at a million).  The normalised k stays in 32 bits up
+// position times the frequency's fraction wraps as the angle does, so far positions lose little: the frequency, from
+// 64-bit floating point, is off by up to 2^-54 of a turn a position, and the angle's rounding to fp32 adds 2^-26 of a turn
+// (a float product is off by 2^-24 of the angle, 0.06 rad at a million).  The normalised k stays in 32 bits up
 // to its one rounding, the quantisation.
 constexpr int kPrepThreads = 256, kPrepRows = 2;
 

@@ -47,8 +47,8 @@ typedef struct dflash_kv_cache {
  * q_out row r (bf16, stride ld_q; may be qkv itself with ld_q = ld) = RMSNorm (q_norm) and
  * rotary embedding of the q heads; k heads get k_norm and the rotary embedding and go, like
  * v, to the cache in its format.  Rotary position: position0 (a shared prefix's length, say)
- * + lengths[b] + t, rotate-half on the first rot dims, frequency theta^(-2i/rot), angles
- * exact to 2^-30 of a turn at any position.  parents (NULL, or device int32
+ * + lengths[b] + t, rotate-half on the first rot dims, frequency theta^(-2i/rot), angles off
+ * by at most 2^-26 + position 2^-54 of a turn.  parents (NULL, or device int32
  * [sequences, tokens], tokens <= 32): each block is a speculative tree and t becomes the
  * row's depth.  Quantisation keeps the affine rule of the weights: the edge of a group with
  * the larger magnitude is stored exactly (as a bf16 bias), the code of zero is a whole
