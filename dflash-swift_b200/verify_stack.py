@@ -738,6 +738,7 @@ class VerifyStack:
                 n += 2 + 1 + 1 + 1 + 2  # in_proj, conv + gates, gdn_step, gated_norm, out_proj
             else:
                 n += 2 + 1 + 1 + 2  # qkv, prep, decode, o_proj
+                n += self.kv_bits is not None  # the batch entry joins its parts in a kernel of its own
             n += 2 + 2  # gate_up, down (SwiGLU inside its prep; pushes inside the qmm epilogues)
         return n
 
@@ -893,7 +894,7 @@ def main(argv=None) -> int:
             "tp": world, "steps": args.steps, "warmup": args.warmup,
             "weight_bytes_per_gpu": wbytes, "weight_gbs_per_gpu": round(wbytes / (ms / 1000.0) / 1e9, 1),
             "kernels_per_forward": stack.kernels_per_forward(), "all_reduces_per_forward": 2 * cfg.layers,
-            "allreduce": stack.allreduce, "tree": None if args.tree is None else stack.tree_plan.parents,
+            "allreduce": stack.allreduce, "kv_bits": args.kv_bits, "tree": None if args.tree is None else stack.tree_plan.parents,
             "config": {k: v for k, v in asdict(cfg).items()}, "out_abs_sum": checksum,
         }), flush=True)
     del g

@@ -136,3 +136,11 @@ def test_the_binding_refuses_a_stream_of_another_device(dc):
     stream = SimpleNamespace(device=torch.device("cuda", 1))
     with pytest.raises(ValueError, match="stream"):
         dc._elsewhere(torch.device("cuda", 0), stream)
+
+
+def test_a_stack_over_batch_caches_counts_its_launches():
+    """Attention over them is two kernels a layer, over the single-sequence caches one."""
+    import verify_stack as vs
+    count = lambda bits: vs.VerifyStack.kernels_per_forward(SimpleNamespace(cfg=vs.TINY, kv_bits=bits))  # noqa: E731
+    layers = sum(1 for k in vs.TINY.layer_kinds() if k != "gdn")
+    assert layers > 0 and count(8) == count(16) == count(None) + layers
