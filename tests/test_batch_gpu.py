@@ -632,3 +632,31 @@ def test_the_stack_over_a_batch_cache(dc, cuda, bits, bar, tree):
     assert dc.device_error() == 0
     with pytest.raises(ValueError):
         new.advance(100)
+
+
+@pytest.mark.parametrize("bits,group,bar", [(4, 64, 0.18), (4, 32, 0.18), (8, 32, 3e-2)])
+def test_the_stack_over_smaller_caches_and_groups(dc, cuda, bits, group, bar):
+    """As above with 4 bits, whose half step is 16 times that of 8 (2e-2 + 16 (3e-2 - 2e-2)), and groups of 32."""
+    import verify_stack as vs
+    cfg = vs.TINY
+    caches = replace(cfg, block=24)
+    plan = vs.shard_plan(cfg, 0, 1)
+    weights = vs.build_rank_weights(cfg, plan, 0, cuda)
+    new = vs.VerifyStack(cfg, device=cuda, weights=weights, state=vs.build_rank_state(caches, plan, 0, cuda), kv_bits=bits,
+                         kv_group=group)
+    state = vs.build_rank_state(caches, plan, 0, cuda)
+    for S, N in zip(state["layers"], new.state["layers"]):
+        if "cache" in N:
+            assert (N["cache"].bits, N["cache"].group) == (bits, group)
+            k, v = dc.stack_kv_read(N["cache"], N["cache"].max_len)
+            S["cache_k"].copy_(k[0])
+            S["cache_v"].copy_(v[0])
+    old = vs.VerifyStack(cfg, device=cuda, weights=weights, state=state)
+    hidden = vs.make_block(cfg, 0, cuda)
+    for _ in range(2):
+        a, b = new.forward(hidden).float(), old.forward(hidden).float()
+        assert (a - b).abs().max() <= bar * b.abs().max()
+        for s in (new, old):
+            s.commit([0, 1, 2])
+            s.advance(3)
+    assert dc.device_error() == 0
