@@ -14,8 +14,13 @@
 //   O^T [d x rows]        += V^T [d x 128] P^T         V as it lies in the cache, read transposed
 // so few rows waste nothing (a product costs as long as reading its 128-row operand from shared
 // memory up to 64 rows), no operand is transposed by a thread, and a thread that reads S^T owns
-// one key: its mask and its scale factors are its own registers.  Q, K, V and P are bf16 over bf16
-// caches.  Over quantised caches they are fp16, whose 11 bits lose little to the codes' 8: every
+// one key: its mask and its scale factors are its own registers.
+//
+// Q, K, V and P are bf16 over bf16 caches: a product takes one type for both operands, and the cache's range is not fp16's.
+// P's rounding to 2^-9 is the price (0.0023 of the output against 64 bits, where the output's own rounding is 0.0017 and
+// dflash_stack_attn_decode's fp32 weights add nothing).  P in two parts would cost half as much product again and 32 KB of
+// shared memory, one of three ring slots at 256 dims; a sum of the rounded P gained nothing (0.0023) and took 2 % more time.
+// Over quantised caches they are fp16, whose 11 bits lose little to the codes' 8: every
 // key's values (and every query row) are first scaled by a power of two into fp16's upper range,
 // undone in S^T for K and Q, and for V folded into P's exponent and the sum's weights.
 //
@@ -26,11 +31,12 @@
 // kLazy (in powers of two), so the accumulators are rarely rescaled.
 //
 // Measured in a captured graph, join included (256 dims, 24 q heads on 4 kv heads, groups of 64): a block of 8 tokens
-// over 1024 rows of 8 bits 17.5 us; over 131071 rows 103 us (2.8 TB/s; HBM alone would take 44); 33 sequences of one token
-// over about 4096 rows of 4 bits 92 us; 64 sequences of 4 tokens that share 32768 bf16 rows 254 us (0.81 PFLOP/s); with
-// 128 dims, 16 q heads on 2 kv heads, 2 x 509 tokens over about 7000 rows of 8 bits 150 us.  Over quantised caches no
-// unit is full (131071 rows: instructions, mostly the unpack's and the softmax's, take 52 % of the issue slots, shared memory's
-// banks are 30 % busy, the tensor cores 17 %): the chain from codes to boxes to S to P to O, which two or three slots
+// over 1024 rows of 8 bits 18.4 us; over 131071 rows 107 us (2.7 TB/s; HBM alone would take 44); 33 sequences of one token
+// over about 4096 rows of 4 bits 93 us; 64 sequences of 4 tokens that share 32768 bf16 rows 245 us (0.84 PFLOP/s) in a
+// short run, 265 to 280 us once the GPU has been under such load for a second (graph and call alike); with
+// 128 dims, 16 q heads on 2 kv heads, 2 x 509 tokens over about 7000 rows of 8 bits 149 us.  Over quantised caches no
+// unit is full (131071 rows: instructions, mostly the unpack's and the softmax's, take 56 % of the issue slots, shared memory's
+// banks are 29 % busy, the tensor cores 16 %): the chain from codes to boxes to S to P to O, which two or three slots
 // overlap only in part, bounds it.  Over bf16 caches the products take about half of a tile's time, the rest is the same
 // chain and the change of units.  Both have some 25 us beside their tiles: launch, first loads, the changes of units
 // (5 us each) and the join (11 us there).
@@ -56,9 +62,11 @@ constexpr int kMaxCtas = 160;              // partials are sized for this many C
 constexpr int kMaxSlots = 10;              // ring slots: two boxes each, one where d is 64
 constexpr int kMaxStages = 8;              // staging slots for codes: 64 or 128 rows each
 constexpr int kScaleDepth = 2;             // tiles whose key factors may be alive at once
-// Tiles that take as long as the change to another unit, about.  64 sequences of 200 rows behind a bf16 prefix of 32768: 451 us
-// with none, 287 with 1, 295 with 2, 254 with 4, 308 with 6; 32 of 250 rows behind 8190 of 8 bits: 47.3, 40.5, 41.0, 47.5 with
-// none, 1, 2 and 4 (long sequences: 92.7, 93.2, 92.1, 91.4).
+// Tiles that the change to another unit of a sequence counts as in the plan.  Counting none leaves SMs with many short units
+// far behind; beyond that the number was picked from two shapes, is not monotone (it moves the runs' borders), and weighs a
+// tile of few rows like one of 128 and a change within the prefix as nothing.  64 sequences of 200 rows behind a bf16 prefix of
+// 32768: 451 us with none, 287 with 1, 295 with 2, 254 with 4, 308 with 6; 32 of 250 rows behind 8190 of 8 bits: 47.3, 40.5,
+// 41.0, 47.5 with none, 1, 2 and 4 (long sequences: 92.7, 93.2, 92.1, 91.4).
 __host__ __device__ constexpr int unit_cost(int bits) { return bits == 16 ? 4 : 2; }
 constexpr int kPoison = 16;                // units whose poison flags may be alive at once
 constexpr float kLazy = 4.f;               // a maximum moves when a score passes it by 2^4 ...

@@ -153,7 +153,9 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // kSettle have been found the threshold is the top-th of those; where even kCandidates had no room for a
 // round's (a row that ascends), the round is looked at again under the new threshold.
 // 509 bf16 rows of 248320 logits with eight alternatives take 91 us in a graph (2.8 TB/s; HBM alone would take 39): bound by
-// issue (a conversion, a comparison, an exponential and two sums for each logit) and by the last wave's few rows.  Few rows are bound by latency: 8 of them 14.7 us.
+// issue (a conversion, a comparison, an exponential and two sums for each logit), by two block barriers a round with no load
+// in flight, and by uneven SMs (509 rows are one wave of CTAs, three rows on some SMs and four on others).  Few rows are bound
+// by latency: 8 of them 14.7 us.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(
     const T* __restrict__ logits, long long ld, int vocab, const int32_t* __restrict__ tokens, int n, int top,

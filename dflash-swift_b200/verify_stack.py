@@ -356,7 +356,9 @@ class VerifyStack:
 
     kv_bits (16, 8 or 4): the attention layers run on the batch entries (dflash_batch.h) over
     a dflashcuda.KVCache of that many bits in groups of kv_group, filled from the bf16 caches
-    of `state`, which the stack then no longer holds; the position is device-resident."""
+    of `state`, which the stack then no longer holds; the position is device-resident.  kv_bits=16 is
+    not the default path to the bit: the batch entry rounds the weights of a row to bf16
+    (dflash_stack_attn_decode keeps them in fp32)."""
 
     def __init__(self, cfg: StackConfig, rank: int = 0, world: int = 1, seed: int = 0, device=None,
                  group=None, weights: Optional[dict] = None, state: Optional[dict] = None, allreduce: str = "peer",

@@ -91,8 +91,10 @@ int dflash_stack_kv_compact_batch(const dflash_kv_cache* cache, const int32_t* l
  * and hq * d).  The prefix has the cache's bits, group, kv_heads and head_dim, sequences = 1.
  * Cache rows that a token does not see never reach its output, whatever they hold.  Over
  * quantised caches the operands are fp16, each row scaled by a power of two: an element under
- * 2^-11 (8 bits) or 2^-7 (4 bits) of its row's largest is held to 2^-22 or 2^-18 of that one, and
- * the rows of V that a token sees may differ in size by 2^126 (a row of zeros counts as 2^-62).
+ * 2^-11 (8 bits) or 2^-7 (4 bits) of its row's largest is held to 2^-22 or 2^-18 of that one, a
+ * weight under 2^-22 of the token's largest (weight times size of its V row) to 2^-33 of that one,
+ * and the rows of V that a token sees may differ in size by 2^126 (a row of zeros counts as 2^-62).
+ * Over bf16 caches weights are rounded to bf16 before the product with V (not in their sum).
  * workspace: dflash_stack_attn_decode_batch_workspace_bytes() bytes of device memory, 16-byte
  * aligned, contents irrelevant before and after; calls that may run at the same time need one
  * each.  The size depends on the arguments only, not on the lengths; 0: not supported.
